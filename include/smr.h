@@ -375,6 +375,67 @@ int smr_set_gemv_launch(int threads_per_row, int sub_shards);
  * to rounding, not bit for bit.  Process-wide. */
 int smr_set_gemv_matrix_cores(int on);
 
+/* The end of a tensor-parallel block: the one-shot all-reduce of its partial sums fused with
+ * the norm behind the block, its gate, the scaled residual and the norm in front of the next
+ * block.  No reference code; the reduce and its handshake are one_shot_all_reduce's
+ * (symm_mem_recipes/triton_one_shot_all_reduce.py:59-93).  For every row:
+ *   s = ((0 + buf_0) + buf_1) + ... + buf_{ws-1}              fp32
+ *   n = s * (mean(s^2) + eps)^-1/2 * post_weight              (post_weight NULL: n = s)
+ *   h = residual_scale * residual + gate * n
+ *   residual_out = h;  normed = h * (mean(h^2) + eps)^-1/2 * weight;  summed = s (NULL: not wanted)
+ * Everything between the loads and the stores is fp32; each output is rounded once.
+ *   buffer_ptrs_host, signal_pad_ptrs_host  HOST arrays, as in smr_one_shot_all_reduce_addrs
+ *              (pads NULL allowed with SMR_BARRIER_NONE); every buffer holds rows * cols elements,
+ *              each pad 4096 * world_size slots
+ *   dtype      SMR_DTYPE_BF16 or _FP32, of all tensors; rows are contiguous, cols in 1..16384
+ *   gate_kind  0 none (gate NULL), 1 one per column [cols], 2 one per row [rows], 3 [rows, cols]
+ *   barrier_mode  SMR_BARRIER_NONE or _PROXY.  residual_out may be residual. */
+int smr_all_reduce_norm(const uint64_t* buffer_ptrs_host, const uint64_t* signal_pad_ptrs_host, const void* residual,
+                        const void* weight, const void* post_weight, const void* gate, int gate_kind, void* normed,
+                        void* residual_out, void* summed, int64_t rows, int64_t cols, int dtype, double residual_scale,
+                        double eps, int rank, int world_size, int barrier_mode, uint32_t* status, void* stream);
+
+/* Its backward pass from `summed` and `residual_out` of the forward one and the gradients of its
+ * two outputs (grad_residual_out NULL: zero).  grad_partial is the gradient of every rank's
+ * partial sums.  Gradients of the weights and of a broadcast gate are summed over what they were
+ * broadcast over, in fp32 and in an order that depends on the sizes only.
+ *   scratch    smr_norm_backward_scratch_bytes(...) bytes; needs no initialisation */
+int smr_norm_backward(const void* grad_normed, const void* grad_residual_out, const void* summed,
+                      const void* residual_out, const void* weight, const void* post_weight, const void* gate,
+                      int gate_kind, void* grad_partial, void* grad_residual, void* grad_weight,
+                      void* grad_post_weight, void* grad_gate, float* scratch, int64_t scratch_bytes, int64_t rows,
+                      int64_t cols, int dtype, double residual_scale, double eps, void* stream);
+int64_t smr_norm_backward_scratch_bytes(int64_t rows, int64_t cols, int has_post_weight, int gate_kind);
+
+/* 4-bit microscaled operands (OCP MXFP4: e2m1 elements, one e8m0 scale per 32 along the
+ * contracted axis), no reference code; the next narrower form of its FP8_OUTPUT switch
+ * (symm_mem_recipes/triton_all_gather_matmul.py:115,123).  An operand of `rows` rows and `cols`
+ * of the contracted axis is two arrays in the order the MFMA takes them, units of 16 rows x 256:
+ *   codes   [ceil(rows/16)][ceil(cols/256)][2 steps][64 lanes][16 B]; lane l of a step holds row
+ *           l & 15, elements 32 * (l >> 4) .. + 31 of the step's 128, the first of a pair in the
+ *           low half of its byte
+ *   scales  [ceil(rows/16)][ceil(cols/256)][64 lanes][2 steps] biased exponents, 255 = NaN
+ * with zeros where a unit reaches past rows or cols. */
+int64_t smr_mxfp4_code_bytes(int64_t rows, int64_t cols);
+int64_t smr_mxfp4_scale_bytes(int64_t rows, int64_t cols);
+
+/* x [rows, cols] (dtype SMR_DTYPE_BF16 or _FP32, row_stride elements from row to row) -> codes and
+ * scales, blocks of 32 along the rows of x; transpose 1: along its columns, the result then is
+ * the operand of x^T (cols rows, contracted axis rows).
+ *   scale = 2^(floor(log2(max |block|)) - 2), at least 2^-127; elements round to nearest even and
+ *   saturate at 6 scales.  A block that holds an infinity or a NaN becomes NaN (scale code 255). */
+int smr_mxfp4_quantize(const void* x_dev, int64_t row_stride, void* codes_dev, void* scales_dev, int64_t rows,
+                       int64_t cols, int dtype, int transpose, void* stream);
+/* The values an operand stands for, [rows, cols] contiguous bf16 or fp32 (exact in both). */
+int smr_mxfp4_dequantize(const void* codes_dev, const void* scales_dev, void* out_dev, int64_t rows, int64_t cols,
+                         int dtype, void* stream);
+
+/* C[M,N] = A[M,K] * B[N,K]^T of two such operands, fp32 accumulation, C contiguous bf16 or fp32
+ * (out_dtype).  A NaN block makes NaN what it takes part in. */
+int smr_mxfp4_matmul(const void* a_codes_dev, const void* a_scales_dev, const void* b_codes_dev,
+                     const void* b_scales_dev, void* c_dev, int64_t M, int64_t N, int64_t K, int out_dtype,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -28,7 +28,7 @@ STATUS_TEXT = {
     ST_MISMATCH: "signal-round checksum mismatch",
 }
 
-_p, _i, _i64, _u32 = C.c_void_p, C.c_int, C.c_int64, C.c_uint32
+_p, _i, _i64, _u32, _d = C.c_void_p, C.c_int, C.c_int64, C.c_uint32, C.c_double
 
 # name -> (restype, argtypes); mirrors include/smr.h one to one
 SIGNATURES = {
@@ -69,6 +69,14 @@ SIGNATURES = {
     "smr_gemv_flag_words": (_i, [_i, _i, _i]),
     "smr_set_gemv_launch": (_i, [_i, _i]),
     "smr_set_gemv_matrix_cores": (_i, [_i]),
+    "smr_all_reduce_norm": (_i, [_p, _p, _p, _p, _p, _p, _i, _p, _p, _p, _i64, _i64, _i, _d, _d, _i, _i, _i, _p, _p]),
+    "smr_norm_backward": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _d, _d, _p]),
+    "smr_norm_backward_scratch_bytes": (_i64, [_i64, _i64, _i, _i]),
+    "smr_mxfp4_code_bytes": (_i64, [_i64, _i64]),
+    "smr_mxfp4_scale_bytes": (_i64, [_i64, _i64]),
+    "smr_mxfp4_quantize": (_i, [_p, _i64, _p, _p, _i64, _i64, _i, _i, _p]),
+    "smr_mxfp4_dequantize": (_i, [_p, _p, _p, _i64, _i64, _i, _p]),
+    "smr_mxfp4_matmul": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p]),
 }
 
 _lib: Optional[C.CDLL] = None

@@ -1,0 +1,171 @@
+"""4-bit microscaled operands (OCP MXFP4: e2m1 elements, one power-of-two scale per 32 of
+them along the contracted axis): quantisation, the values back, and the product of two
+operands.  The next narrower form of the e4m3fn switch of the all-gather matmul
+(symm_mem_recipes/triton_all_gather_matmul.py:115,123,188), which has no 4-bit form.
+
+For training, the two products of a linear layer's backward pass contract over the layer's
+outputs and over the tokens; ``mxfp4_quantize(..., transpose=True)`` gives their operands::
+
+    y  = mxfp4_matmul(x, mxfp4_quantize(w))                       # x [T, K], w [N, K]
+    dx = mxfp4_matmul(dy, mxfp4_quantize(w, transpose=True))      # contracts over N
+    dw = mxfp4_matmul(mxfp4_quantize(dy, transpose=True),         # contracts over T
+                      mxfp4_quantize(x, transpose=True))
+"""
+from __future__ import annotations
+
+from typing import Optional, Union
+
+import torch
+
+from . import _lib
+
+#: elements that share a scale; rows and contracted extent of a storage unit
+BLOCK, UNIT_ROWS, SLAB = 32, 16, 256
+
+_DTYPE_CODE = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_FP32}
+#: the current stream's handle without building a torch.cuda.Stream object around it
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _call(device: torch.device, what: str, fn, *args) -> None:
+    """``fn(*args, stream)`` on ``device``'s current stream, with ``device`` current."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc != 0:
+        _lib.check(rc, what)
+
+
+class MxFp4Tensor:
+    """A matrix ``[rows, cols]`` in 4-bit microscaled floats, ``cols`` the axis that a product
+    contracts, kept in the order the matrix cores take it (``smr.h``: ``smr_mxfp4_code_bytes``).
+    Made by :func:`mxfp4_quantize` or :meth:`from_blocks`; it owns ``codes`` and ``scales``."""
+
+    __slots__ = ("codes", "scales", "rows", "cols")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
+        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((self.rows, self.cols))
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def __repr__(self) -> str:
+        return f"MxFp4Tensor(rows={self.rows}, cols={self.cols}, device={self.device})"
+
+    @staticmethod
+    def empty(rows: int, cols: int, device) -> "MxFp4Tensor":
+        """Storage for a matrix, its values undefined."""
+        rows, cols = int(rows), int(cols)
+        assert 0 <= rows < 2 ** 31 and 1 <= cols < 2 ** 31, "rows must be in 0..2^31-1, cols in 1..2^31-1"
+        units = -(-rows // UNIT_ROWS) * -(-cols // SLAB)
+        return MxFp4Tensor(torch.empty(units * 2048, dtype=torch.uint8, device=device),
+                           torch.empty(units * 128, dtype=torch.uint8, device=device), rows, cols)
+
+    @staticmethod
+    def from_blocks(codes: torch.Tensor, scales: torch.Tensor, cols: Optional[int] = None) -> "MxFp4Tensor":
+        """From the layout checkpoints use: ``codes`` uint8 [rows, blocks * 16], two elements a
+        byte, the first in the low half, and ``scales`` uint8 [rows, blocks] biased exponents,
+        a block being 32 columns.  ``cols`` (default: blocks * 32) says how many columns are
+        real; what the last block holds past them is taken as zero."""
+        assert codes.dtype == torch.uint8 and scales.dtype == torch.uint8, "codes and scales must be uint8"
+        assert codes.dim() == 2 and scales.dim() == 2 and codes.shape[0] == scales.shape[0]
+        assert codes.device == scales.device, "codes and scales must be on one device"
+        rows, blocks = scales.shape
+        assert codes.shape[1] == blocks * (BLOCK // 2), "codes must have 16 bytes per block"
+        cols = blocks * BLOCK if cols is None else int(cols)
+        assert blocks >= 1 and blocks == -(-cols // BLOCK), "cols must end in the last block"
+        row_units, slabs = -(-rows // UNIT_ROWS), -(-cols // SLAB)
+        padded = torch.zeros(row_units * UNIT_ROWS, slabs * SLAB // 2, dtype=torch.uint8, device=codes.device)
+        used = -(-cols // 2)
+        padded[:rows, :used] = codes[:, :used]
+        if cols % 2:
+            padded[:rows, used - 1] &= 15
+        padded = padded.view(row_units, UNIT_ROWS, slabs, 2, 4, 16)          # unit row, row, slab, step, block, byte
+        exponents = torch.zeros(row_units * UNIT_ROWS, slabs * 8, dtype=torch.uint8, device=codes.device)
+        exponents[:rows, :blocks] = scales
+        exponents = exponents.view(row_units, UNIT_ROWS, slabs, 2, 4)
+        return MxFp4Tensor(padded.permute(0, 2, 3, 4, 1, 5).contiguous().view(-1),
+                           exponents.permute(0, 2, 4, 1, 3).contiguous().view(-1), rows, cols)
+
+    def to_blocks(self):
+        """``(codes, scales)`` in the layout :meth:`from_blocks` takes."""
+        row_units, slabs = -(-self.rows // UNIT_ROWS), -(-self.cols // SLAB)
+        blocks = -(-self.cols // BLOCK)
+        codes = self.codes.view(row_units, slabs, 2, 4, UNIT_ROWS, 16).permute(0, 4, 1, 2, 3, 5)
+        scales = self.scales.view(row_units, slabs, 4, UNIT_ROWS, 2).permute(0, 3, 1, 4, 2)
+        return (codes.reshape(row_units * UNIT_ROWS, slabs * SLAB // 2)[:self.rows, :blocks * 16].contiguous(),
+                scales.reshape(row_units * UNIT_ROWS, slabs * 8)[:self.rows, :blocks].contiguous())
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The values, ``[rows, cols]`` bf16 or fp32 (exact in both)."""
+        if out is None:
+            assert dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
+            out = torch.empty(self.rows, self.cols, dtype=dtype, device=self.codes.device)
+        else:
+            assert out.dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
+            assert tuple(out.shape) == (self.rows, self.cols) and out.is_contiguous(), "out must be contiguous [rows, cols]"
+            assert out.device == self.codes.device, "out must be on the operand's device"
+        assert out.is_cuda, "the operand must be on a GPU"
+        _call(out.device, "mxfp4_dequantize", _lib.load().smr_mxfp4_dequantize, self.codes.data_ptr(),
+              self.scales.data_ptr(), out.data_ptr(), self.rows, self.cols, _DTYPE_CODE[out.dtype])
+        return out
+
+
+def mxfp4_quantize(x: torch.Tensor, *, transpose: bool = False, out: Optional[MxFp4Tensor] = None) -> MxFp4Tensor:
+    """``x`` [rows, cols] bf16 or fp32, elements of a row adjacent (rows may be apart), in 4-bit
+    microscaled floats with blocks of 32 along its rows.
+
+    ``transpose`` blocks along the columns: the operand of ``x.T``, for products that contract
+                  over ``x``'s rows.
+    ``out``       storage of the result's shape to write into.
+
+    A block's scale is ``2 ** (floor(log2(max |block|)) - 2)``, at least 2^-127; its elements round
+    to nearest even and saturate at 6 scales.  A block with an infinity or a NaN becomes NaN."""
+    assert x.dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
+    assert x.dim() == 2, "x must be a matrix"
+    rows, cols = x.shape
+    assert cols <= 1 or x.stride(1) == 1, "the elements of a row must be adjacent"
+    row_stride = x.stride(0) if rows > 1 else cols
+    assert row_stride >= cols, "the rows of x must not overlap"
+    shape = (cols, rows) if transpose else (rows, cols)
+    assert x.is_cuda, "x must be on a GPU"
+    if out is None:
+        out = MxFp4Tensor.empty(shape[0], shape[1], x.device)
+    else:
+        assert (out.rows, out.cols) == shape, "out has another shape"
+        assert out.codes.device == x.device, "out must be on x's device"
+    _call(x.device, "mxfp4_quantize", _lib.load().smr_mxfp4_quantize, x.data_ptr(), row_stride,
+          out.codes.data_ptr(), out.scales.data_ptr(), rows, cols, _DTYPE_CODE[x.dtype], 1 if transpose else 0)
+    return out
+
+
+def mxfp4_matmul(a: Union[MxFp4Tensor, torch.Tensor], b: MxFp4Tensor, *, out_dtype: torch.dtype = torch.bfloat16,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``a @ b.T`` for ``a`` [M, K] and ``b`` [N, K], accumulated in fp32 and rounded once to
+    ``out_dtype`` (bf16 or fp32).  A bf16 or fp32 ``a`` is quantised on the way
+    (:func:`mxfp4_quantize`; the result is the same)."""
+    assert isinstance(b, MxFp4Tensor), "b must be an MxFp4Tensor"
+    assert len(a.shape) == 2 and a.shape[1] == b.cols, "a and b must be matrices with one contracted extent"
+    device = b.codes.device
+    assert a.device == device, "a and b must be on one device"
+    assert device.type == "cuda", "the operands must be on a GPU"
+    if not isinstance(a, MxFp4Tensor):
+        a = mxfp4_quantize(a)
+    if out is None:
+        assert out_dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
+        out = torch.empty(a.rows, b.rows, dtype=out_dtype, device=device)
+    else:
+        assert out.dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
+        assert tuple(out.shape) == (a.rows, b.rows) and out.is_contiguous(), "out must be contiguous [M, N]"
+        assert out.device == device, "out must be on the operands' device"
+    _call(device, "mxfp4_matmul", _lib.load().smr_mxfp4_matmul, a.codes.data_ptr(), a.scales.data_ptr(),
+          b.codes.data_ptr(), b.scales.data_ptr(), out.data_ptr(), a.rows, b.rows, a.cols, _DTYPE_CODE[out.dtype])
+    return out

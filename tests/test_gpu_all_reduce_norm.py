@@ -1,0 +1,284 @@
+"""The all-reduce fused with norms, gate and residual, and its backward pass, on the GPU against
+64-bit arithmetic."""
+import pytest
+import torch
+
+from tests import norm_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+def _gate_shape(kind, shape):
+    return {"none": None, "channel": shape[-1:], "token": tuple(shape[:-1]) + (1,), "element": tuple(shape)}[kind]
+
+
+def _inputs(shape, ranks, dtype, post, gate, seed):
+    gen = torch.Generator().manual_seed(seed)
+    rand = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    shape = tuple(shape)
+    partials = rand(ranks, *shape).to(dtype)
+    residual = (rand(*shape) * torch.exp(0.5 * rand(shape[-1]))).to(dtype)
+    weight = (1 + 0.1 * rand(shape[-1])).to(dtype)
+    post_weight = (1 + 0.1 * rand(shape[-1])).to(dtype) if post else None
+    gate_shape = _gate_shape(gate, shape)
+    gate = None if gate_shape is None else (0.5 + 0.3 * rand(*gate_shape)).to(dtype)
+    return partials, residual, weight, post_weight, gate
+
+
+def _symmetric(partials, rank):
+    from symm_mem_recipes import EmulatedSymmetricMemory as SM
+    ranks, shape = partials.shape[0], tuple(partials.shape[1:])
+    strides, step = [], 1
+    for n in reversed(shape):
+        strides.insert(0, step)
+        step *= n
+    t = SM.empty_strided_p2p(shape, strides, partials.dtype, "cuda", world_size=ranks, rank=rank)
+    for r in range(ranks):
+        SM.rendezvous(t).get_buffer(r, shape, partials.dtype).copy_(partials[r])
+    return t, SM.rendezvous(t)
+
+
+def _cuda(*tensors):
+    return [None if t is None else t.cuda() for t in tensors]
+
+
+def _within(got, want, off, dtype):
+    """Half a step of the result's type, of the value that is rounded."""
+    half = torch.finfo(dtype).eps / 2
+    bound = (want.abs() + off) * half + off + torch.finfo(dtype).tiny
+    d = (got.cpu().double() - want).abs()
+    assert got.dtype == dtype and got.shape == want.shape
+    assert bool((d <= bound).all()), (float((d - bound).max()), int((d > bound).sum()))
+
+
+FORWARD = [
+    # shape, ranks, dtype, post, gate, scale
+    ((1, 8), 1, "bf16", True, "none", 1.0), ((1, 1), 2, "fp32", True, "channel", 1.0), ((5,), 3, "bf16", True, "channel", 0.5),
+    ((1, 8192), 8, "bf16", True, "channel", 1.25), ((2, 3, 64), 8, "bf16", False, "token", 1.0),
+    ((3, 1000), 5, "bf16", True, "element", -0.5), ((4, 1001), 7, "bf16", True, "token", 1.0),
+    ((7, 1001), 5, "fp32", True, "element", 1.0), ((3, 63), 4, "fp32", False, "none", 0.0),
+    ((300, 96), 8, "bf16", True, "channel", 1.0), ((600, 512), 2, "bf16", False, "channel", 1.0),
+    ((2, 8200), 8, "bf16", True, "element", 1.0), ((2, 16384), 4, "bf16", True, "none", 1.0),
+    ((2, 16383), 3, "bf16", True, "token", 1.0), ((2, 16381), 2, "fp32", True, "channel", 1.0),
+    ((1030, 2048), 6, "bf16", True, "token", 1.0), ((5000, 40), 8, "fp32", True, "element", 1.0),
+]
+
+
+@pytest.mark.parametrize("shape,ranks,dtype,post,gate,scale", FORWARD)
+def test_forward(cuda, shape, ranks, dtype, post, gate, scale):
+    from symm_mem_recipes import EmulatedSymmetricMemory as SM, one_shot_all_reduce_norm
+    dtype = DTYPES[dtype]
+    partials, residual, weight, post_weight, g = _inputs(shape, ranks, dtype, post, gate, sum(shape) + ranks)
+    t, handle = _symmetric(partials, rank=ranks - 1)
+    x, w, p, gc = _cuda(residual, weight, post_weight, g)
+    kw = dict(post_weight=p, gate=gc, residual_scale=scale, eps=1e-5)
+    got = one_shot_all_reduce_norm(t, x, w, return_sum=True, **kw)
+    want = oracle.forward(partials, residual, weight, post_weight, g, scale, 1e-5)
+    off = oracle.forward_bounds(partials, residual, weight, post_weight, g, scale, 1e-5)
+    for a, b, c in zip(got, want, off):
+        _within(a, b, c, dtype)
+    for _ in range(2):
+        again = one_shot_all_reduce_norm(t, x, w, return_sum=True, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(got, again))
+    without = one_shot_all_reduce_norm(t, x, w, barrier=False, **kw)
+    assert len(without) == 2 and all(torch.equal(a, b) for a, b in zip(got, without))
+    handle.check_status()
+    assert all(int(handle.get_signal_pad(r).abs().sum()) == 0 for r in range(ranks))
+    for r in range(ranks):
+        assert torch.equal(handle.get_buffer(r, shape, dtype).cpu(), partials[r])        # the inputs stay
+    SM.release()
+
+
+def test_the_sum_is_one_shot_all_reduce(cuda):
+    from symm_mem_recipes import EmulatedSymmetricMemory as SM, one_shot_all_reduce, one_shot_all_reduce_norm
+    for dtype in DTYPES.values():
+        partials, residual, weight, post_weight, _ = _inputs((33, 1024), 8, dtype, True, "none", 9)
+        t, _ = _symmetric(partials, 2)
+        x, w, p = _cuda(residual, weight, post_weight)
+        _, _, s = one_shot_all_reduce_norm(t, x, w, post_weight=p, return_sum=True)
+        assert torch.equal(s, one_shot_all_reduce(t))
+    SM.release()
+
+
+def test_rows_of_zeros_infinities_and_nan(cuda):
+    """A row of zeros divides by sqrt(eps) and stays zero; an infinity or NaN spoils its own row
+    and no other."""
+    from symm_mem_recipes import EmulatedSymmetricMemory as SM, one_shot_all_reduce_norm
+    partials, residual, weight, post_weight, _ = _inputs((6, 200), 3, torch.bfloat16, True, "none", 1)
+    partials[:, 0] = 0
+    residual[0] = 0
+    partials[1, 2, 7] = float("inf")
+    residual[4, 199] = float("nan")
+    t, _ = _symmetric(partials, 0)
+    y, h = one_shot_all_reduce_norm(t, residual.cuda(), weight.cuda(), post_weight=post_weight.cuda())
+    assert bool((y[0] == 0).all()) and bool((h[0] == 0).all())
+    clean = [1, 3, 5]
+    want = oracle.forward(partials, residual, weight, post_weight, None, 1.0, 1e-6)
+    off = oracle.forward_bounds(partials, residual, weight, post_weight, None, 1.0, 1e-6)
+    for got, b, c in zip((y, h), want, off):
+        _within(got[clean], b[clean], c[clean], torch.bfloat16)
+    assert bool(y[2].isnan().any()) and bool(y[4].isnan().all())
+    SM.release()
+
+
+def test_large_values_do_not_overflow_before_the_type_does(cuda):
+    from symm_mem_recipes import EmulatedSymmetricMemory as SM, one_shot_all_reduce_norm
+    partials, residual, weight, post_weight, _ = _inputs((2, 256), 2, torch.float32, True, "none", 3)
+    partials, residual = partials * 1e15, residual * 1e15
+    t, _ = _symmetric(partials, 0)
+    got = one_shot_all_reduce_norm(t, residual.cuda(), weight.cuda(), post_weight=post_weight.cuda())
+    args = (partials, residual, weight, post_weight, None, 1.0, 1e-6)
+    for a, b, c in zip(got, oracle.forward(*args), oracle.forward_bounds(*args)):
+        _within(a, b, c, torch.float32)
+    SM.release()
+
+
+def test_no_tokens(cuda):
+    from symm_mem_recipes import EmulatedSymmetricMemory as SM, one_shot_all_reduce_norm, one_shot_all_reduce_norm_backward
+    t = SM.empty_strided_p2p((0, 64), (64, 1), torch.bfloat16, "cuda", world_size=4, rank=0)
+    x, w = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    y, h, s = one_shot_all_reduce_norm(t, x, w, return_sum=True)
+    assert y.shape == h.shape == s.shape == (0, 64)
+    g = one_shot_all_reduce_norm_backward(y, h, s, h, w, post_weight=w, gate=w)
+    assert g.partial.shape == (0, 64) and not g.weight.any() and not g.post_weight.any() and not g.gate.any()
+    SM.release()
+
+
+BACKWARD = [
+    ((1, 8), "bf16", True, "none", 1.0, True), ((1, 1), "fp32", True, "channel", 1.0, True), ((5,), "bf16", True, "channel", 0.5, True),
+    ((5, 4096), "bf16", False, "none", 1.25, True), ((2, 3, 64), "bf16", False, "token", 1.0, True),
+    ((3, 1000), "bf16", True, "element", -0.5, False), ((4, 1001), "bf16", True, "token", 1.0, True),
+    ((7, 1001), "fp32", True, "element", 1.0, True), ((3, 63), "fp32", False, "channel", 0.0, False),
+    ((300, 96), "bf16", True, "channel", 1.0, True), ((600, 512), "fp32", True, "channel", 1.0, True),
+    ((2, 8200), "bf16", True, "element", 1.0, True), ((2, 16384), "bf16", True, "channel", 1.0, True),
+    ((2, 16383), "bf16", True, "token", 1.0, True), ((2, 16381), "fp32", True, "channel", 1.0, True),
+    ((1030, 2048), "bf16", True, "token", 1.0, True), ((5000, 40), "fp32", True, "element", 1.0, True),
+]
+
+
+def _backward_inputs(shape, dtype, post, gate, with_dh, seed):
+    _, h, weight, post_weight, g = _inputs(shape, 1, dtype, post, gate, seed)
+    gen = torch.Generator().manual_seed(seed + 1)
+    s, dy, dh = (torch.randn(*shape, generator=gen).to(dtype) for _ in range(3))
+    return dy, dh if with_dh else None, s * 2, h, weight, post_weight, g
+
+
+@pytest.mark.parametrize("shape,dtype,post,gate,scale,with_dh", BACKWARD)
+def test_backward(cuda, shape, dtype, post, gate, scale, with_dh):
+    """Every term of a gradient passes through at most 128 roundings on its way (32 values and 22
+    partial sums in each of two row sums, the rest single operations); a column sum adds at most
+    rows / 256 terms in a workgroup, 16 of each thread's and 16 threads'."""
+    from symm_mem_recipes import one_shot_all_reduce_norm_backward
+    dtype = DTYPES[dtype]
+    args = _backward_inputs(shape, dtype, post, gate, with_dh, sum(shape))
+    dy, dh, s, h, w, p, g = _cuda(*args)
+    got = one_shot_all_reduce_norm_backward(dy, dh, s, h, w, post_weight=p, gate=g, residual_scale=scale, eps=1e-5)
+    want = oracle.backward(*args, scale, 1e-5)
+    size = oracle.backward(*args, scale, 1e-5, magnitudes=True)
+    assert (got.post_weight is None) == (not post) and (got.gate is None) == (gate == "none")
+    rows = dy.numel() // dy.shape[-1]
+    for name, b in want.items():
+        a = getattr(got, name)
+        off = size[name] * (128 + rows / 256 + 32) * oracle.U
+        _within(a.reshape(b.shape), b, off, dtype)
+    again = one_shot_all_reduce_norm_backward(dy, dh, s, h, w, post_weight=p, gate=g, residual_scale=scale, eps=1e-5)
+    assert all(a is None and b is None or torch.equal(a, b) for a, b in zip(got, again))
+
+
+def test_backward_against_differences(cuda):
+    """Every gradient against central differences of the 64-bit forward pass, through fp32
+    inputs: the loss is a weighted sum of both outputs."""
+    from symm_mem_recipes import one_shot_all_reduce_norm_backward
+    gen = torch.Generator().manual_seed(5)
+    rand = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    T, H, scale, eps = 3, 10, 0.75, 1e-3
+    for gate_shape in ((H,), (T, 1), (T, H)):
+        leaves = {"partial": rand(T, H), "residual": rand(T, H), "weight": 1 + 0.1 * rand(H), "post_weight": 1 + 0.1 * rand(H),
+                  "gate": 0.5 + 0.3 * rand(*gate_shape)}
+        dy, dh = rand(T, H), rand(T, H)
+
+        def loss(v):
+            y, h, _ = oracle.forward(v["partial"][None], v["residual"], v["weight"], v["post_weight"], v["gate"], scale, eps)
+            return float((y * dy.double()).sum() + (h * dh.double()).sum())
+
+        _, h, s = oracle.forward(leaves["partial"][None], leaves["residual"], leaves["weight"], leaves["post_weight"],
+                                 leaves["gate"], scale, eps)
+        got = one_shot_all_reduce_norm_backward(dy.cuda(), dh.cuda(), s.float().cuda(), h.float().cuda(), leaves["weight"].cuda(),
+                                                post_weight=leaves["post_weight"].cuda(), gate=leaves["gate"].cuda(),
+                                                residual_scale=scale, eps=eps)
+        step = 1e-5           # error of a central difference: step^2 * (third derivative) ~ 1e-9, 64-bit rounding ~ 1e-10
+        for name, leaf in leaves.items():
+            grad = getattr(got, name).cpu().double()
+            for i in range(leaf.numel()):
+                up, down = ({k: v.double().clone() for k, v in leaves.items()} for _ in range(2))
+                up[name].view(-1)[i] += step
+                down[name].view(-1)[i] -= step
+                slope = (loss(up) - loss(down)) / (2 * step)
+                # fp32 inputs h and s and fp32 arithmetic: 200 roundings of terms of order 10
+                assert abs(float(grad.view(-1)[i]) - slope) <= 200 * oracle.U * 10 + 1e-6, (name, i)
+
+
+def test_graphs_replay_the_forward_and_the_backward_pass(cuda):
+    """Two captured graphs on one allocation's signal pads, eager calls and synchronisations in
+    between; each replay is checked against the eager result for the inputs of the moment."""
+    from symm_mem_recipes import (EmulatedSymmetricMemory as SM, one_shot_all_reduce_norm,
+                                  one_shot_all_reduce_norm_backward)
+    partials, residual, weight, post_weight, g = _inputs((40, 520), 8, torch.bfloat16, True, "channel", 2)
+    t, handle = _symmetric(partials, 3)
+    x, w, p, gc = _cuda(residual, weight, post_weight, g)
+    kw = dict(post_weight=p, gate=gc)
+
+    def both():
+        y, h, s = one_shot_all_reduce_norm(t, x, w, return_sum=True, **kw)
+        return (y, h, s) + tuple(one_shot_all_reduce_norm_backward(y, h, s, h, w, **kw))
+
+    both()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = both()
+        graphs.append((graph, out))
+    for turn in range(3):
+        for graph, out in graphs:
+            x.copy_(torch.randn(40, 520) * (turn + 1))
+            graph.replay()
+            torch.cuda.synchronize()
+            want = both()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+    handle.check_status()
+    SM.release()
+
+
+def test_a_layer_boundary(cuda):
+    """The operators together as a layer uses them: reduce, norms, gate and residual, then the
+    next product in 4 bits - for one token and for a prompt - and the way back."""
+    from symm_mem_recipes import (EmulatedSymmetricMemory as SM, mxfp4_matmul, mxfp4_quantize, one_shot_all_reduce_norm,
+                                  one_shot_all_reduce_norm_backward)
+    from tests import mxfp4_oracle as mx
+    for T in (1, 150):
+        H, N = 512, 320
+        partials, residual, weight, post_weight, g = _inputs((T, H), 8, torch.bfloat16, True, "channel", T)
+        w_next = (torch.randn(N, H, generator=torch.Generator().manual_seed(T)) * H ** -0.5).bfloat16()
+        t, handle = _symmetric(partials, 0)
+        x, w, p, gc, wn = _cuda(residual, weight, post_weight, g, w_next)
+        y, h, s = one_shot_all_reduce_norm(t, x, w, post_weight=p, gate=gc, return_sum=True)
+        out = mxfp4_matmul(y, mxfp4_quantize(wn))
+        y64, w64 = mx.values(*mx.quantize(y)), mx.values(*mx.quantize(w_next))
+        want = y64 @ w64.t()
+        bound = want.abs() * 2.0 ** -8 + (H + 16) * oracle.U * (y64.abs() @ w64.abs().t()) * 1.01
+        assert bool(((out.cpu().double() - want).abs() <= bound).all())
+        d_out = torch.randn(T, N, generator=torch.Generator().manual_seed(7)).bfloat16().cuda()
+        dy = mxfp4_matmul(d_out, mxfp4_quantize(wn, transpose=True))
+        dw = mxfp4_matmul(mxfp4_quantize(d_out, transpose=True), mxfp4_quantize(y, transpose=True))
+        assert dy.shape == (T, H) and dw.shape == (N, H)
+        got = one_shot_all_reduce_norm_backward(dy, None, s, h, w, post_weight=p, gate=gc)
+        args = (dy.cpu(), None, s.cpu(), h.cpu(), weight, post_weight, g, 1.0, 1e-6)
+        want, size = oracle.backward(*args), oracle.backward(*args, magnitudes=True)
+        for name, b in want.items():
+            _within(getattr(got, name).reshape(b.shape), b, size[name] * (128 + 32) * oracle.U, torch.bfloat16)
+        handle.check_status()
+    SM.release()
