@@ -411,10 +411,10 @@ int64_t smr_norm_backward_scratch_bytes(int64_t rows, int64_t cols, int has_post
  * contracted axis), no reference code; the next narrower form of its FP8_OUTPUT switch
  * (symm_mem_recipes/triton_all_gather_matmul.py:115,123).  An operand of `rows` rows and `cols`
  * of the contracted axis is two arrays in the order the MFMA takes them, units of 16 rows x 256:
- *   codes   [ceil(rows/16)][ceil(cols/256)][2 steps][64 lanes][16 B]; lane l of a step holds row
+ *   codes   [ceil(cols/256)][ceil(rows/16)][2 steps][64 lanes][16 B]; lane l of a step holds row
  *           l & 15, elements 32 * (l >> 4) .. + 31 of the step's 128, the first of a pair in the
  *           low half of its byte
- *   scales  [ceil(rows/16)][ceil(cols/256)][64 lanes][2 steps] biased exponents, 255 = NaN
+ *   scales  [ceil(cols/256)][ceil(rows/16)][64 lanes][2 steps] biased exponents, 255 = NaN
  * with zeros where a unit reaches past rows or cols. */
 int64_t smr_mxfp4_code_bytes(int64_t rows, int64_t cols);
 int64_t smr_mxfp4_scale_bytes(int64_t rows, int64_t cols);
@@ -435,6 +435,15 @@ int smr_mxfp4_dequantize(const void* codes_dev, const void* scales_dev, void* ou
 int smr_mxfp4_matmul(const void* a_codes_dev, const void* a_scales_dev, const void* b_codes_dev,
                      const void* b_scales_dev, void* c_dev, int64_t M, int64_t N, int64_t K, int out_dtype,
                      void* stream);
+
+/* smr_mxfp4_matmul for a few rows of A still in bf16 or fp32 (x [M, K], row_stride elements from row
+ * to row), quantised on the way; the result is bit for bit that of smr_mxfp4_quantize followed by
+ * smr_mxfp4_matmul.  M up to smr_mxfp4_matmul_rows_limit(K): 16, fewer beyond K = 5632, none beyond
+ * 90112 (they are kept in LDS). */
+int64_t smr_mxfp4_matmul_rows_limit(int64_t K);
+int smr_mxfp4_matmul_rows(const void* x_dev, int64_t row_stride, int dtype, const void* b_codes_dev,
+                          const void* b_scales_dev, void* c_dev, int64_t M, int64_t N, int64_t K, int out_dtype,
+                          void* stream);
 
 #ifdef __cplusplus
 }

@@ -345,14 +345,6 @@ static bool norm_shape(int cols, int vec, int max_threads, int& threads, int& ch
   return false;
 }
 
-static int compute_units() {
-  int dev = 0, cus = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1)
-    return 256;
-  return cus;
-}
-
 // Workgroups of a backward launch (each leaves cols fp32 sums per kind).
 static int backward_blocks(int64_t rows) {
   const int64_t cap = 256;

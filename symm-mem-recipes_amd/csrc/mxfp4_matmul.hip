@@ -11,9 +11,6 @@ namespace smr {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 // D += A x B over 128 of K; `step` picks the byte of the scale words that belongs to it.
 template <int STEP>
@@ -25,30 +22,30 @@ __device__ __forceinline__ f32x4 mfma_mx(const i32x4& first, const i32x4& second
                                                           (int)second_scale);
 }
 
-// Four consecutive columns n .. n+3 of row m.
+// Four consecutive columns of a row, all of them there.
+template <bool BF16>
+__device__ __forceinline__ void put4(uint8_t* p, const f32x4& d) {
+  if constexpr (BF16) {
+    const u32x2 v = {pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3])};
+    *reinterpret_cast<u32x2_any*>(p) = v;
+  } else {
+    const u32x4 v = {__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2]), __float_as_uint(d[3])};
+    *reinterpret_cast<u32x4_any*>(p) = v;
+  }
+}
+// Columns n .. n+3 of row m, as far as they exist.
 template <bool BF16>
 __device__ __forceinline__ void store4(uint8_t* c, int64_t m, int64_t n, int64_t N, const f32x4& d) {
   const int64_t at = m * N + n;
-  if constexpr (BF16) {
-    const u32x2 v = {pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3])};
-    uint16_t* p = reinterpret_cast<uint16_t*>(c) + at;
-    if (n + 4 <= N) {
-      *reinterpret_cast<u32x2_any*>(p) = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < N) p[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-    }
+  if (n + 4 <= N) {
+    put4<BF16>(c + at * (BF16 ? 2 : 4), d);
   } else {
-    float* p = reinterpret_cast<float*>(c) + at;
-    if (n + 4 <= N) {
-      const u32x4_any v = {__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2]), __float_as_uint(d[3])};
-      *reinterpret_cast<u32x4_any*>(p) = v;
-    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < N) p[e] = d[e];
-    }
+    for (int e = 0; e < 4; ++e)
+      if (n + e < N) {
+        if constexpr (BF16) reinterpret_cast<uint16_t*>(c)[at + e] = (uint16_t)f32_to_bf16_bits(d[e]);
+        else reinterpret_cast<float*>(c)[at + e] = d[e];
+      }
   }
 }
 
@@ -61,51 +58,61 @@ __global__ __launch_bounds__(WAVES * 64) void mxfp4_matmul_few_kernel(
     const uint8_t* __restrict__ b_scales, uint8_t* __restrict__ c, int64_t M, int64_t N, int64_t slabs,
     int64_t m_units, int64_t n_units) {
   __shared__ f32x4 part[WAVES][NG * TG][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  // in a scalar register: branches on it are scalar ones (a matrix instruction does not look at the
+  // lanes' mask, so it must not stand under one)
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int64_t n_unit0 = (int64_t)blockIdx.x * NG, m_unit0 = (int64_t)blockIdx.y * TG;
-  const uint8_t *ac[TG], *as[TG], *bc[NG], *bs[NG];
+  // Uniform addresses (units past the last repeat it; their products are not stored) and a lane's
+  // offset: the loads then need no address arithmetic per lane.
+  const uint32_t code_at = lane * 16, scale_at = lane * 2;
+  int64_t au[TG], bu[NG];
 #pragma unroll
-  for (int t = 0; t < TG; ++t) {
-    // (units past the last repeat it; their products are not stored)
-    const int64_t u = (m_unit0 + t < m_units ? m_unit0 + t : m_units - 1) * slabs;
-    ac[t] = a_codes + u * kMxCodeBytes + lane * 16;
-    as[t] = a_scales + u * kMxScaleBytes + lane * 2;
-  }
+  for (int t = 0; t < TG; ++t) au[t] = m_unit0 + t < m_units ? m_unit0 + t : m_units - 1;
 #pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    const int64_t u = (n_unit0 + g < n_units ? n_unit0 + g : n_units - 1) * slabs;
-    bc[g] = b_codes + u * kMxCodeBytes + lane * 16;
-    bs[g] = b_scales + u * kMxScaleBytes + lane * 2;
-  }
+  for (int g = 0; g < NG; ++g) bu[g] = n_unit0 + g < n_units ? n_unit0 + g : n_units - 1;
   f32x4 acc[NG][TG];
 #pragma unroll
   for (int g = 0; g < NG; ++g)
 #pragma unroll
     for (int t = 0; t < TG; ++t) acc[g][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-#pragma unroll 2
-  for (int64_t s = wave; s < slabs; s += WAVES) {
-    i32x4 bf[NG][2], af[TG][2];
-    uint32_t bsc[NG], asc[TG];
+  struct Slab {
+    i32x4 b[NG][2], a[TG][2];
+    uint32_t bs[NG], as[TG];
+  };
+  auto load = [&](Slab& v, int64_t s) __attribute__((always_inline)) {
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      bf[g][0] = *reinterpret_cast<const i32x4*>(bc[g] + s * kMxCodeBytes);
-      bf[g][1] = *reinterpret_cast<const i32x4*>(bc[g] + s * kMxCodeBytes + 1024);
-      bsc[g] = *reinterpret_cast<const uint16_t*>(bs[g] + s * kMxScaleBytes);
+      const uint8_t* p = b_codes + (s * n_units + bu[g]) * kMxCodeBytes;
+      v.b[g][0] = *reinterpret_cast<const i32x4*>(p + code_at);
+      v.b[g][1] = *reinterpret_cast<const i32x4*>(p + 1024 + code_at);
+      v.bs[g] = *reinterpret_cast<const uint16_t*>(b_scales + (s * n_units + bu[g]) * kMxScaleBytes + scale_at);
     }
 #pragma unroll
     for (int t = 0; t < TG; ++t) {
-      af[t][0] = *reinterpret_cast<const i32x4*>(ac[t] + s * kMxCodeBytes);
-      af[t][1] = *reinterpret_cast<const i32x4*>(ac[t] + s * kMxCodeBytes + 1024);
-      asc[t] = *reinterpret_cast<const uint16_t*>(as[t] + s * kMxScaleBytes);
+      const uint8_t* p = a_codes + (s * m_units + au[t]) * kMxCodeBytes;
+      v.a[t][0] = *reinterpret_cast<const i32x4*>(p + code_at);
+      v.a[t][1] = *reinterpret_cast<const i32x4*>(p + 1024 + code_at);
+      v.as[t] = *reinterpret_cast<const uint16_t*>(a_scales + (s * m_units + au[t]) * kMxScaleBytes + scale_at);
     }
+  };
+  auto multiply = [&](const Slab& v) __attribute__((always_inline)) {
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
-      for (int t = 0; t < TG; ++t) {
-        acc[g][t] = mfma_mx<0>(bf[g][0], af[t][0], acc[g][t], bsc[g], asc[t]);
-        acc[g][t] = mfma_mx<1>(bf[g][1], af[t][1], acc[g][t], bsc[g], asc[t]);
-      }
+      for (int t = 0; t < TG; ++t) acc[g][t] = mfma_mx<0>(v.b[g][0], v.a[t][0], acc[g][t], v.bs[g], v.as[t]);
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int t = 0; t < TG; ++t) acc[g][t] = mfma_mx<1>(v.b[g][1], v.a[t][1], acc[g][t], v.bs[g], v.as[t]);
+  };
+  // (a second and third slab in flight per wave gained nothing: with eight waves the loads of one fill
+  // the path to the compute unit)
+  for (int64_t s = wave; s < slabs; s += WAVES) {
+    Slab v;
+    load(v, s);
+    multiply(v);
   }
 #pragma unroll
   for (int g = 0; g < NG; ++g)
@@ -127,6 +134,589 @@ __global__ __launch_bounds__(WAVES * 64) void mxfp4_matmul_few_kernel(
   }
 }
 
+// The same for the product of a few rows that are still bf16 or fp32 (generation: one launch instead
+// of two, and no operand written and read back).  Every workgroup quantises all of them into LDS, a
+// block of 32 per thread - its share of B is on the way meanwhile - and goes on as above; the lanes of
+// rows that do not exist repeat the last one.
+template <bool BF16, bool XBF16, int NG, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void mxfp4_matmul_rows_kernel(
+    const uint8_t* __restrict__ x, int64_t row_bytes, const uint8_t* __restrict__ b_codes,
+    const uint8_t* __restrict__ b_scales, uint8_t* __restrict__ c, int M, int64_t N, int64_t K, int slabs,
+    int64_t n_units) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t rows_lds[];
+  __shared__ f32x4 part[WAVES][NG][64];
+  // codes [slabs * 8 blocks][M][16 B], then scales [slabs][4][M][2 steps]
+  i32x4* codes = reinterpret_cast<i32x4*>(rows_lds);
+  uint8_t* scales = rows_lds + (size_t)slabs * 8 * M * 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int64_t n_unit0 = (int64_t)blockIdx.x * NG;
+  const uint32_t code_at = lane * 16, scale_at = lane * 2;
+  int64_t bu[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) bu[g] = n_unit0 + g < n_units ? n_unit0 + g : n_units - 1;
+  struct Slab {
+    i32x4 b[NG][2];
+    uint32_t bs[NG];
+  };
+  auto load = [&](Slab& v, int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const uint8_t* p = b_codes + (s * n_units + bu[g]) * kMxCodeBytes;
+      v.b[g][0] = *reinterpret_cast<const i32x4*>(p + code_at);
+      v.b[g][1] = *reinterpret_cast<const i32x4*>(p + 1024 + code_at);
+      v.bs[g] = *reinterpret_cast<const uint16_t*>(b_scales + (s * n_units + bu[g]) * kMxScaleBytes + scale_at);
+    }
+  };
+  Slab next;
+  load(next, wave < slabs ? wave : slabs - 1);
+
+  const int blocks = slabs * 8;
+  for (int i = threadIdx.x; i < blocks * M; i += WAVES * 64) {
+    const int r = i / blocks, b = i - r * blocks;
+    const uint8_t* p = x + r * row_bytes + (int64_t)b * 32 * Mx8<XBF16>::kSize;
+    const int64_t left = K - (int64_t)b * 32;
+    Mx8<XBF16> v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j].load(p + j * 8 * Mx8<XBF16>::kSize, left - j * 8);
+    const uint32_t code = mx_scale_code(mx_top<XBF16>(v));
+    const float scale = mx_scale_value(code);
+    i32x4 w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = code == 255u ? 0 : (int)mx_pack8<XBF16>(v[j], scale);
+    codes[b * M + r] = w;
+    scales[((((b >> 3) * 4 + (b & 3)) * M) + r) * 2 + ((b >> 2) & 1)] = (uint8_t)code;
+  }
+  __syncthreads();
+
+  f32x4 acc[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) acc[g] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const int row = (lane & 15) < M ? (lane & 15) : M - 1;
+  for (int s = wave; s < slabs; s += WAVES) {
+    const Slab v = next;
+    load(next, s + WAVES < slabs ? s + WAVES : s);
+    const i32x4 a0 = codes[(s * 8 + (lane >> 4)) * M + row], a1 = codes[(s * 8 + 4 + (lane >> 4)) * M + row];
+    const uint32_t as = *reinterpret_cast<const uint16_t*>(scales + ((s * 4 + (lane >> 4)) * M + row) * 2);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) acc[g] = mfma_mx<0>(v.b[g][0], a0, acc[g], v.bs[g], as);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) acc[g] = mfma_mx<1>(v.b[g][1], a1, acc[g], v.bs[g], as);
+  }
+#pragma unroll
+  for (int g = 0; g < NG; ++g) part[wave][g][lane] = acc[g];
+  __syncthreads();
+  for (int g = wave; g < NG; g += WAVES) {
+    f32x4 d = part[0][g][lane];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+      const f32x4 p = part[w][g][lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[e] += p[e];
+    }
+    const int64_t n = (n_unit0 + g) * kMxRows + (lane >> 4) * 4;
+    if ((lane & 15) < M && n < N) store4<BF16>(c, lane & 15, n, N, d);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The tiled kernel, for products with enough rows to fill matrix tiles: a persistent grid of
+// 256-thread workgroups, one per compute unit, each computing BM x BN tiles with 4 waves in a
+// 2 x 2 arrangement.  A slab (rows x 256 of K, 128 bytes a row) comes from memory straight into
+// LDS with 128-bit direct-to-LDS loads; operands being in MFMA order, loads and fragment reads
+// are both linear.  LDS holds three slabs of A, two of B and two sets of scales: while one pair
+// of slabs is multiplied, the next is complete or landing and the A slab after that is on its
+// way.  With the bf16 MFMA replaced by one that does four times the work on the same bytes in
+// the same time, the bytes per cycle are those of the bf16 GEMM of ag_matmul.hip, and so is the
+// order of work inside a slab pair (two steps of 128 of K):
+//   first step    MFMAs of step 0; the fragments of step 1 are read; A slab kt+2 is requested
+//   barrier       pair kt is read by everyone, pair kt+1 has landed
+//   second step   MFMAs of step 1; fragments of step 0 and the scales of pair kt+1 are read;
+//                 B slab and scales of pair kt+2 are requested
+typedef __attribute__((address_space(3))) void LdsVoid;
+
+constexpr int kTileThreads = 256;
+
+__device__ __forceinline__ i32x4 lds_frag(uint32_t addr) {
+  return *reinterpret_cast<__attribute__((address_space(3))) const i32x4*>((uintptr_t)addr);
+}
+__device__ __forceinline__ uint16_t lds_u16(uint32_t addr) {
+  return *reinterpret_cast<__attribute__((address_space(3))) const uint16_t*>((uintptr_t)addr);
+}
+// A pointer that is the same in every lane, kept in scalar registers.
+__device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
+  const uint64_t v = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return (const uint8_t*)(uintptr_t)(((uint64_t)hi << 32) | lo);
+}
+// 1 KiB from memory to LDS: lane l's 16 bytes at base + voff land at lds_dst + 16 l.  In assembly so that the
+// compiler does not count it: it would make every fragment read wait for it.  All waits for these
+// loads are the explicit vmcnt below (loads return in order).
+__device__ __forceinline__ void load_kib(const uint8_t* base, uint32_t voff, uint32_t lds_dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds_dst), "v"(voff), "s"(base)
+               : "memory", "m0");
+}
+// D += A x B with the accumulator named as an accumulation register, so that the compiler does not
+// move the accumulators between the register files inside the loop.  STEP picks the byte of the
+// scale registers.
+template <int STEP>
+__device__ __forceinline__ void mfma_mx_acc(f32x4& acc, const i32x4& first, const i32x4& second, uint16_t first_scale,
+                                            uint16_t second_scale) {
+  if constexpr (STEP == 0)
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                 : "+a"(acc)
+                 : "v"(first), "v"(second), "v"(first_scale), "v"(second_scale));
+  else
+    asm volatile(
+        "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+        : "+a"(acc)
+        : "v"(first), "v"(second), "v"(first_scale), "v"(second_scale));
+}
+// The same with a load_kib behind it.  With one wave per SIMD an instruction between two MFMAs costs
+// an issue slot, and an MFMA lasts four of them: the write of M0 stands ahead of the MFMA, which is
+// the distance the load needs from it.
+template <int STEP, int OFFSET>
+__device__ __forceinline__ void mfma_mx_load(f32x4& acc, const i32x4& first, const i32x4& second, uint16_t first_scale,
+                                             uint16_t second_scale, const uint8_t* base, uint32_t voff,
+                                             uint32_t lds_dst) {
+  if constexpr (STEP == 0)
+    asm volatile(
+        "s_add_i32 m0, %5, %6\n\t"
+        "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t"
+        "global_load_lds_dwordx4 %7, %8"
+        : "+a"(acc)
+        : "v"(first), "v"(second), "v"(first_scale), "v"(second_scale), "s"(lds_dst), "i"(OFFSET), "v"(voff), "s"(base)
+        : "memory", "m0", "scc");
+  else
+    asm volatile(
+        "s_add_i32 m0, %5, %6\n\t"
+        "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t"
+        "global_load_lds_dwordx4 %7, %8"
+        : "+a"(acc)
+        : "v"(first), "v"(second), "v"(first_scale), "v"(second_scale), "s"(lds_dst), "i"(OFFSET), "v"(voff), "s"(base)
+        : "memory", "m0", "scc");
+}
+
+// Where the other instructions of a step go: every LOAD_GAP-th of the first MFMAs carries a load, and
+// `reads` LDS reads are spread over the MFMAs in between among the first SPAN, one each.
+// The read behind MFMA `at` (the MFMA-th slot), or -1.
+template <int LOADS, int LOAD_GAP, int READS, int SPAN>
+struct StepPlan {
+  static constexpr bool is_load(int at) { return at % LOAD_GAP == 0 && at / LOAD_GAP < LOADS; }
+  static constexpr int free_before(int at) {
+    int n = 0;
+    for (int i = 0; i < at; ++i) n += !is_load(i);
+    return n;
+  }
+  static constexpr int kFree = free_before(SPAN);
+  // reads first .. last - 1 go behind MFMA `at`
+  static constexpr int first(int at) {
+    if constexpr (kFree == 0) return at == 0 ? 0 : READS;         // (tiles of a few MFMAs)
+    else return at >= SPAN ? READS : (free_before(at) * READS + kFree - 1) / kFree;
+  }
+};
+template <int I>
+struct Index {
+  static constexpr int value = I;
+};
+// f(Index<0>), ..., f(Index<N - 1>): a loop whose counter is a constant in every turn
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void unrolled(F&& f) {
+  if constexpr (I < N) {
+    f(Index<I>{});
+    unrolled<N, I + 1>(f);
+  }
+}
+
+struct MxTiles {
+  const uint8_t *a_codes, *a_scales, *b_codes, *b_scales;
+  uint8_t* c;
+  int64_t M, N;
+  int slabs, m_units, n_units;
+  int tiles_m, tiles_n, group_m;
+};
+
+// Tile number `lin` of the order: groups of group_m row tiles, column by column inside a group.
+__device__ __forceinline__ void mx_tile_at(const MxTiles& t, int lin, int& tile_m, int& tile_n) {
+  const int per_group = t.group_m * t.tiles_n;
+  const int first = lin / per_group * t.group_m;
+  const int rows = t.tiles_m - first < t.group_m ? t.tiles_m - first : t.group_m;
+  const int in_group = lin % per_group;
+  tile_m = first + in_group % rows;
+  tile_n = in_group / rows;
+}
+
+// The tile of workgroup `wg` in pass `pass` over the grid, -1 if it has none: within a pass XCD x
+// (workgroups with wg % 8 == x) takes a contiguous run of the tile order, a patch about as wide
+// as it is high, so that the workgroups that share an L2 share rows of A and B.
+__device__ __forceinline__ int mx_tile_number(int total, int grid, int wg, int pass) {
+  const int64_t start = (int64_t)pass * grid;
+  if (start >= total) return -1;
+  const int count = total - start < grid ? (int)(total - start) : grid;
+  const int per_xcd = (count + 7) >> 3;
+  const int at = (wg & 7) * per_xcd + (wg >> 3);
+  return (wg >> 3) < per_xcd && at < count ? (int)start + at : -1;
+}
+
+// A wave's FM x FN fragments to rows m0.., columns n0.. of C.
+template <bool BF16, int FM, int FN>
+__device__ __forceinline__ void store_tile(const MxTiles& p, int64_t m0, int64_t n0, int lane, const f32x4 (&acc)[FN][FM]) {
+  constexpr int kSize = BF16 ? 2 : 4;
+  const int64_t m_lane = m0 + (lane & 15), n_lane = n0 + (lane >> 4) * 4;
+  if (n0 + FN * 16 <= p.N) {
+    // all columns exist: one address per row of fragments, the columns are immediate offsets
+    uint8_t* out = p.c + (m_lane * p.N + n_lane) * kSize;
+#pragma unroll
+    for (int mi = 0; mi < FM; ++mi) {
+      if (m_lane + mi * 16 < p.M) {
+#pragma unroll
+        for (int ni = 0; ni < FN; ++ni) put4<BF16>(out + ni * 16 * kSize, acc[ni][mi]);
+      }
+      out += p.N * (16 * kSize);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  } else {
+#pragma unroll
+    for (int mi = 0; mi < FM; ++mi) {
+#pragma unroll
+      for (int ni = 0; ni < FN; ++ni)
+        if (m_lane + mi * 16 < p.M && n_lane + ni * 16 < p.N)
+          store4<BF16>(p.c, m_lane + mi * 16, n_lane + ni * 16, p.N, acc[ni][mi]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+template <bool BF16, int BM, int BN>
+__global__ __launch_bounds__(kTileThreads, 1) void mxfp4_matmul_tile_kernel(MxTiles p) {
+  constexpr int FM = BM / 32, FN = BN / 32;             // 16 x 16 fragments per wave, either way
+  constexpr int GA = BM / 32, GB = BN / 32;             // 1 KiB loads per wave and slab
+  constexpr int kA = BM * 128, kB = BN * 128;           // bytes of a slab
+  constexpr int SA = (BM / 16 + 7) / 8, SB = (BN / 16 + 7) / 8;        // 1 KiB loads of scales (8 units each)
+  constexpr int kS = (SA + SB) * 1024;
+  constexpr int kOffB = 3 * kA, kOffS = kOffB + 2 * kB;
+  static_assert(SA + SB <= 4, "one load of scales per wave");
+  static_assert(kOffS + 2 * kS <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kOffS + 2 * kS];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(LdsVoid*)lds;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int wm = wave >> 1, wn = wave & 1;
+  const int nk = p.slabs;
+  // from one slab of an operand to the next
+  const int64_t a_step = (int64_t)p.m_units * kMxCodeBytes, b_step = (int64_t)p.n_units * kMxCodeBytes;
+  const int total = p.tiles_m * p.tiles_n;
+
+  const uint8_t *a_base, *b_base, *s_base;
+  uint32_t a_off[GA], b_off[GB], s_off;
+  // Addresses of a tile's loads.  Units past the last repeat it: they feed results nobody stores.
+  auto aim = [&](int tile_m, int tile_n) {
+    const int mu = tile_m * (BM / 16), nu = tile_n * (BN / 16);
+    a_base = uniform_ptr(p.a_codes + (int64_t)mu * kMxCodeBytes);
+    b_base = uniform_ptr(p.b_codes + (int64_t)nu * kMxCodeBytes);
+    const int a_last = p.m_units - 1 - mu, b_last = p.n_units - 1 - nu;
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+#pragma unroll
+    for (int j = 0; j < GA; ++j) {
+      const int q = wave * GA + j, u = (q >> 1) < a_last ? (q >> 1) : a_last;
+      a_off[j] = (uint32_t)u * kMxCodeBytes + (uint32_t)((q & 1) * 1024 + ln * 16);
+    }
+#pragma unroll
+    for (int j = 0; j < GB; ++j) {
+      const int q = wave * GB + j, u = (q >> 1) < b_last ? (q >> 1) : b_last;
+      b_off[j] = (uint32_t)u * kMxCodeBytes + (uint32_t)((q & 1) * 1024 + ln * 16);
+    }
+    const int g = wave % (SA + SB);
+    if (g < SA) {
+      s_base = uniform_ptr(p.a_scales + (int64_t)mu * kMxScaleBytes);
+      const int u = g * 8 + (ln >> 3);
+      s_off = (uint32_t)(u < a_last ? u : a_last) * kMxScaleBytes + (uint32_t)(ln & 7) * 16;
+    } else {
+      s_base = uniform_ptr(p.b_scales + (int64_t)nu * kMxScaleBytes);
+      const int u = (g - SA) * 8 + (ln >> 3);
+      s_off = (uint32_t)(u < b_last ? u : b_last) * kMxScaleBytes + (uint32_t)(ln & 7) * 16;
+    }
+  };
+  const int64_t s_step = (int64_t)(wave % (SA + SB) < SA ? p.m_units : p.n_units) * kMxScaleBytes;
+  const uint32_t s_dst = lds0 + kOffS + (uint32_t)(wave % (SA + SB)) * 1024;
+  auto prologue = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int k = i < nk ? i : nk - 1;
+#pragma unroll
+      for (int j = 0; j < GA; ++j)
+        load_kib(a_base + k * a_step, a_off[j], lds0 + i * kA + (wave * GA + j) * 1024);
+#pragma unroll
+      for (int j = 0; j < GB; ++j)
+        load_kib(b_base + k * b_step, b_off[j], lds0 + kOffB + i * kB + (wave * GB + j) * 1024);
+      load_kib(s_base + k * s_step, s_off, s_dst + i * kS);
+    }
+  };
+
+  int pass = 0, number = mx_tile_number(total, gridDim.x, blockIdx.x, 0);
+  if (number < 0) return;
+  int tile_m, tile_n;
+  mx_tile_at(p, number, tile_m, tile_n);
+  aim(tile_m, tile_n);
+  prologue();
+  for (;;) {
+    f32x4 acc[FN][FM];
+#pragma unroll
+    for (int ni = 0; ni < FN; ++ni)
+#pragma unroll
+      for (int mi = 0; mi < FM; ++mi) acc[ni][mi] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // (loads and the previous tile's stores do not retire in one order: wait for everything)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    uint32_t a_fr = lds0 + (uint32_t)(wm * FM * 2048 + ln * 16);
+    uint32_t b_fr = lds0 + kOffB + (uint32_t)(wn * FN * 2048 + ln * 16);
+    uint32_t sa_fr = lds0 + kOffS + (uint32_t)(wm * FM * 128 + ln * 2);
+    uint32_t sb_fr = lds0 + kOffS + SA * 1024 + (uint32_t)(wn * FN * 128 + ln * 2);
+    i32x4 af0[FM], bf0[FN], af1[FM], bf1[FN];
+    uint16_t sa[2][FM], sb[2][FN];               // by parity of the slab pair
+#pragma unroll
+    for (int f = 0; f < FM; ++f) af0[f] = lds_frag(a_fr + f * 2048);
+#pragma unroll
+    for (int f = 0; f < FN; ++f) bf0[f] = lds_frag(b_fr + f * 2048);
+#pragma unroll
+    for (int f = 0; f < FM; ++f) sa[0][f] = lds_u16(sa_fr + f * 128);
+#pragma unroll
+    for (int f = 0; f < FN; ++f) sb[0][f] = lds_u16(sb_fr + f * 128);
+
+    // What the trip requests: slab kt + 2, the last one again past the end (into places nobody reads
+    // any more; one code path keeps the accumulators in place).
+    const uint8_t* ap = a_base + (2 < nk ? 2 : nk - 1) * a_step;
+    const uint8_t* bp = b_base + (2 < nk ? 2 : nk - 1) * b_step;
+    const uint8_t* sp = s_base + (2 < nk ? 2 : nk - 1) * s_step;
+    uint32_t a_at = 0;                           // offset of A slab kt in its ring of three
+    uint32_t a_to = lds0 + 2 * kA + wave * (GA * 1024);      // where A slab kt + 2 goes
+
+    constexpr int kMfma = FM * FN, kFrags = FM + FN;
+    using Plan0 = StepPlan<GA, kMfma / GA, kFrags, kMfma * 13 / 16>;
+    constexpr int kGap1 = (kMfma / 2) / GB;
+    using Plan1 = StepPlan<GB + 1, kGap1, 2 * kFrags, kMfma * 15 / 16>;
+    // (the last load of the first step stands at (GA - 1) * (kMfma / GA))
+    constexpr bool kRoom = kMfma - 6 >= kMfma * 13 / 16 && kMfma - 6 > (GA - 1) * (kMfma / GA);
+    constexpr int kBook = kRoom ? kMfma - 6 : kMfma - 1, kBookGap = kRoom ? 1 : 0;
+    auto trip = [&](auto parity, int kt) __attribute__((always_inline)) {
+      constexpr int P = decltype(parity)::value;
+      unrolled<kMfma>([&](auto slot) __attribute__((always_inline)) {
+        constexpr int at = decltype(slot)::value, ni = at / FM, mi = at % FM, g = at / (kMfma / GA);
+        if constexpr (Plan0::is_load(at))
+          mfma_mx_load<0, g * 1024>(acc[ni][mi], bf0[ni], af0[mi], sb[P][ni], sa[P][mi], ap, a_off[g], a_to);
+        else
+          mfma_mx_acc<0>(acc[ni][mi], bf0[ni], af0[mi], sb[P][ni], sa[P][mi]);
+        constexpr int r0 = Plan0::first(at), r1 = Plan0::first(at + 1);
+        unrolled<r1 - r0>([&](auto read) __attribute__((always_inline)) {
+          constexpr int r = r0 + decltype(read)::value;
+          if constexpr (r == 0) bf1[0] = lds_frag(b_fr + 1024);
+          else if constexpr (r <= FM) af1[r - 1] = lds_frag(a_fr + 1024 + (r - 1) * 2048);
+          else bf1[r - FM] = lds_frag(b_fr + 1024 + (r - FM) * 2048);
+        });
+        // the uniform bookkeeping goes between the last MFMAs, behind the step's loads and reads
+        if constexpr (at == kBook) {
+          const uint32_t next = a_at == 2 * kA ? 0 : a_at + kA;
+          a_fr += next - a_at;
+          a_at = next;
+        }
+        if constexpr (at == kBook + kBookGap) a_to = lds0 + wave * (GA * 1024) + (a_at >= kA ? a_at - kA : 2 * kA);
+        if constexpr (at == kBook + 2 * kBookGap) b_fr += P == 0 ? (uint32_t)kB : (uint32_t)-kB;
+        if constexpr (at == kBook + 3 * kBookGap) {
+          sa_fr += P == 0 ? (uint32_t)kS : (uint32_t)-kS;
+          sb_fr += P == 0 ? (uint32_t)kS : (uint32_t)-kS;
+        }
+        if constexpr (at == kBook + 4 * kBookGap) ap += kt + 3 < nk ? a_step : 0;
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      // this wave's loads of pair kt+1 are complete; those of A slab kt+2 may be in flight
+      static_assert(GA == 8 || GA == 4 || GA == 2, "explicit vmcnt below");
+      if constexpr (GA == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      else if constexpr (GA == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+      __syncthreads();
+      unrolled<kMfma>([&](auto slot) __attribute__((always_inline)) {
+        constexpr int at = decltype(slot)::value, ni = at / FM, mi = at % FM, g = at / kGap1;
+        if constexpr (Plan1::is_load(at) && g < GB)
+          mfma_mx_load<1, g * 1024>(acc[ni][mi], bf1[ni], af1[mi], sb[P][ni], sa[P][mi], bp, b_off[g < GB ? g : 0],
+                                    lds0 + kOffB + P * kB + wave * (GB * 1024));
+        else if constexpr (Plan1::is_load(at))
+          mfma_mx_load<1, P * kS>(acc[ni][mi], bf1[ni], af1[mi], sb[P][ni], sa[P][mi], sp, s_off, s_dst);
+        else
+          mfma_mx_acc<1>(acc[ni][mi], bf1[ni], af1[mi], sb[P][ni], sa[P][mi]);
+        // pair kt+1: fragment and scale of B row 0, those of A, the other B rows
+        constexpr int r0 = Plan1::first(at), r1 = Plan1::first(at + 1);
+        unrolled<r1 - r0>([&](auto read) __attribute__((always_inline)) {
+          constexpr int r = r0 + decltype(read)::value, f = r >> 1;
+          if constexpr ((r & 1) == 0) {
+            if constexpr (f == 0) bf0[0] = lds_frag(b_fr);
+            else if constexpr (f <= FM) af0[f - 1] = lds_frag(a_fr + (f - 1) * 2048);
+            else bf0[f - FM] = lds_frag(b_fr + (f - FM) * 2048);
+          } else {
+            if constexpr (f == 0) sb[1 - P][0] = lds_u16(sb_fr);
+            else if constexpr (f <= FM) sa[1 - P][f - 1] = lds_u16(sa_fr + (f - 1) * 128);
+            else sb[1 - P][f - FM] = lds_u16(sb_fr + (f - FM) * 128);
+          }
+        });
+        if constexpr (at == kMfma - 3) bp += kt + 3 < nk ? b_step : 0;
+        if constexpr (at == kMfma - 2) sp += kt + 3 < nk ? s_step : 0;
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    };
+    // two trips per turn of the loop, one for each set of scales; an odd last trip stands behind it
+    int kt = 0;
+    for (; kt + 1 < nk; kt += 2) {
+      trip(Index<0>{}, kt);
+      trip(Index<1>{}, kt + 1);
+    }
+    if (kt < nk) trip(Index<0>{}, kt);
+    // The repeated loads of the last steps must not land on top of the next tile's slabs, and the
+    // last MFMAs (assembly the compiler does not time) must be through before their results are read.
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+    __syncthreads();
+    const int64_t m0 = (int64_t)tile_m * BM + wm * (BM / 2), n0 = (int64_t)tile_n * BN + wn * (BN / 2);
+    number = mx_tile_number(total, gridDim.x, blockIdx.x, ++pass);
+    if (number >= 0) {
+      mx_tile_at(p, number, tile_m, tile_n);
+      aim(tile_m, tile_n);
+      prologue();
+    }
+    int le = lane;
+    asm volatile("" : "+v"(le));
+    store_tile<BF16, FM, FN>(p, m0, n0, le, acc);
+    if (number < 0) return;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The same product in smaller tiles, for results that have too few of the large ones to fill the
+// chip.  What bounds those is the time a slab takes to arrive, so LDS holds BUFFERS whole slab pairs
+// and all but the two being multiplied and read are on their way; the order inside a pair is the compiler's.
+// One tile per workgroup.
+template <bool BF16, int BM, int BN, int BUFFERS>
+__global__ __launch_bounds__(kTileThreads) void mxfp4_matmul_ring_kernel(MxTiles p) {
+  constexpr int FM = BM / 32, FN = BN / 32;
+  constexpr int GA = BM / 32, GB = BN / 32;
+  constexpr int SA = (BM / 16 + 7) / 8, SB = (BN / 16 + 7) / 8;
+  constexpr int kA = BM * 128, kB = BN * 128, kPair = kA + kB + (SA + SB) * 1024;
+  constexpr int kInFlight = (BUFFERS - 2) * (GA + GB + 1);
+  static_assert(SA + SB <= 4 && BUFFERS * kPair <= 160 * 1024 && (BUFFERS - 1) * (GA + GB + 1) < 64, "LDS, loads in flight");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[BUFFERS * kPair];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(LdsVoid*)lds;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int wm = wave >> 1, wn = wave & 1;
+  const int nk = p.slabs;
+  const int number = mx_tile_number(p.tiles_m * p.tiles_n, gridDim.x, blockIdx.x, 0);
+  if (number < 0) return;
+  int tile_m, tile_n;
+  mx_tile_at(p, number, tile_m, tile_n);
+  const int mu = tile_m * (BM / 16), nu = tile_n * (BN / 16);
+  const int a_last = p.m_units - 1 - mu, b_last = p.n_units - 1 - nu;
+
+  const int64_t a_step = (int64_t)p.m_units * kMxCodeBytes, b_step = (int64_t)p.n_units * kMxCodeBytes;
+  const uint8_t* ap = uniform_ptr(p.a_codes + (int64_t)mu * kMxCodeBytes);
+  const uint8_t* bp = uniform_ptr(p.b_codes + (int64_t)nu * kMxCodeBytes);
+  uint32_t a_off[GA], b_off[GB], s_off;
+#pragma unroll
+  for (int j = 0; j < GA; ++j) {
+    const int q = wave * GA + j, u = (q >> 1) < a_last ? (q >> 1) : a_last;
+    a_off[j] = (uint32_t)u * kMxCodeBytes + (uint32_t)((q & 1) * 1024 + lane * 16);
+  }
+#pragma unroll
+  for (int j = 0; j < GB; ++j) {
+    const int q = wave * GB + j, u = (q >> 1) < b_last ? (q >> 1) : b_last;
+    b_off[j] = (uint32_t)u * kMxCodeBytes + (uint32_t)((q & 1) * 1024 + lane * 16);
+  }
+  const int g = wave % (SA + SB);                    // (waves past the last piece of scales repeat one)
+  const bool of_a = g < SA;
+  const uint8_t* sp = uniform_ptr(of_a ? p.a_scales + (int64_t)mu * kMxScaleBytes : p.b_scales + (int64_t)nu * kMxScaleBytes);
+  const int64_t s_step = (int64_t)(of_a ? p.m_units : p.n_units) * kMxScaleBytes;
+  {
+    const int u = (of_a ? g : g - SA) * 8 + (lane >> 3), last = of_a ? a_last : b_last;
+    s_off = (uint32_t)(u < last ? u : last) * kMxScaleBytes + (uint32_t)(lane & 7) * 16;
+  }
+  int loaded = 0;                                    // next pair to request; past the end the last one again
+  auto request = [&](uint32_t at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < GA; ++j) load_kib(ap, a_off[j], at + (wave * GA + j) * 1024);
+#pragma unroll
+    for (int j = 0; j < GB; ++j) load_kib(bp, b_off[j], at + kA + (wave * GB + j) * 1024);
+    load_kib(sp, s_off, at + kA + kB + g * 1024);
+    if (++loaded < nk) {
+      ap += a_step;
+      bp += b_step;
+      sp += s_step;
+    }
+  };
+#pragma unroll
+  for (int b = 0; b < BUFFERS; ++b) request(lds0 + b * kPair);
+
+  f32x4 acc[FN][FM];
+#pragma unroll
+  for (int ni = 0; ni < FN; ++ni)
+#pragma unroll
+    for (int mi = 0; mi < FM; ++mi) acc[ni][mi] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  // Fragments are read a pair ahead, into the other of two register sets.
+  struct Frags {
+    i32x4 a[2][FM], b[2][FN];
+    uint16_t sa[FM], sb[FN];
+  };
+  auto read = [&](Frags& v, uint32_t at) __attribute__((always_inline)) {
+    const uint32_t a_fr = at + (uint32_t)(wm * FM * 2048 + lane * 16);
+    const uint32_t b_fr = at + kA + (uint32_t)(wn * FN * 2048 + lane * 16);
+    const uint32_t sa_fr = at + kA + kB + (uint32_t)(wm * FM * 128 + lane * 2);
+    const uint32_t sb_fr = at + kA + kB + SA * 1024 + (uint32_t)(wn * FN * 128 + lane * 2);
+#pragma unroll
+    for (int f = 0; f < FM; ++f) v.sa[f] = lds_u16(sa_fr + f * 128);
+#pragma unroll
+    for (int f = 0; f < FN; ++f) v.sb[f] = lds_u16(sb_fr + f * 128);
+#pragma unroll
+    for (int step = 0; step < 2; ++step) {
+#pragma unroll
+      for (int f = 0; f < FM; ++f) v.a[step][f] = lds_frag(a_fr + step * 1024 + f * 2048);
+#pragma unroll
+      for (int f = 0; f < FN; ++f) v.b[step][f] = lds_frag(b_fr + step * 1024 + f * 2048);
+    }
+  };
+  uint32_t here = lds0;                              // buffer of pair kt
+  // One pair: its fragments are in `now`; pair kt + 1 goes to `then`, pair kt + BUFFERS into its place.
+  auto turn = [&](const Frags& now, Frags& then) __attribute__((always_inline)) {
+    // this wave's share of pair kt + 1 is there; behind the barrier everyone's is, and everyone has pair kt
+    asm volatile("s_waitcnt vmcnt(%0)" : : "i"(kInFlight) : "memory");
+    __syncthreads();
+    request(here);
+    here = here + kPair < lds0 + BUFFERS * kPair ? here + kPair : lds0;
+    read(then, here);
+#pragma unroll
+    for (int ni = 0; ni < FN; ++ni)
+#pragma unroll
+      for (int mi = 0; mi < FM; ++mi)
+        acc[ni][mi] = mfma_mx<0>(now.b[0][ni], now.a[0][mi], acc[ni][mi], now.sb[ni], now.sa[mi]);
+#pragma unroll
+    for (int ni = 0; ni < FN; ++ni)
+#pragma unroll
+      for (int mi = 0; mi < FM; ++mi)
+        acc[ni][mi] = mfma_mx<1>(now.b[1][ni], now.a[1][mi], acc[ni][mi], now.sb[ni], now.sa[mi]);
+  };
+  Frags even, odd;
+  asm volatile("s_waitcnt vmcnt(%0)" : : "i"((BUFFERS - 1) * (GA + GB + 1)) : "memory");
+  __syncthreads();
+  read(even, lds0);
+  int kt = 0;
+  for (; kt + 1 < nk; kt += 2) {
+    turn(even, odd);
+    turn(odd, even);
+  }
+  if (kt < nk) turn(even, odd);
+  // (LDS is given back when the workgroup ends: nothing may still be landing in it)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  store_tile<BF16, FM, FN>(p, (int64_t)tile_m * BM + wm * (BM / 2), (int64_t)tile_n * BN + wn * (BN / 2), lane, acc);
+}
+
 struct MxOperands {
   const uint8_t *a_codes, *a_scales, *b_codes, *b_scales;
   uint8_t* c;
@@ -138,15 +728,116 @@ static int launch_few(const MxOperands& o, hipStream_t s) {
   const int64_t m_units = mx_row_units(o.M), n_units = mx_row_units(o.N);
   const int64_t gx = (n_units + NG - 1) / NG, gy = (m_units + TG - 1) / TG;
   if (gx > kMxMaxGrid / 4 || gy > 65535) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul: too large for one launch");
-  hipLaunchKernelGGL((mxfp4_matmul_few_kernel<BF16, TG, NG, WAVES>), dim3((unsigned)gx, (unsigned)gy), dim3(WAVES * 64),
-                     0, s, o.a_codes, o.a_scales, o.b_codes, o.b_scales, o.c, o.M, o.N, mx_slabs(o.K), m_units, n_units);
+  hipLaunchKernelGGL((mxfp4_matmul_few_kernel<BF16, TG, NG, WAVES>), dim3((unsigned)gx, (unsigned)gy),
+                     dim3(WAVES * 64), 0, s, o.a_codes, o.a_scales, o.b_codes, o.b_scales, o.c, o.M, o.N,
+                     mx_slabs(o.K), m_units, n_units);
   return check_hip(hipGetLastError(), "smr_mxfp4_matmul launch");
+}
+
+struct MxRows {
+  const uint8_t* x;
+  int64_t row_bytes;
+  const uint8_t *b_codes, *b_scales;
+  uint8_t* c;
+  int64_t M, N, K;
+};
+// Rows times slabs whose codes and scales (136 B each) fit a workgroup's LDS beside the partial sums.
+constexpr int kRowsLdsUnits = 352;
+
+template <bool BF16, bool XBF16, int NG, int WAVES>
+static int launch_rows_as(const MxRows& o, hipStream_t s) {
+  const int64_t n_units = mx_row_units(o.N), slabs = mx_slabs(o.K), grid = (n_units + NG - 1) / NG;
+  if (grid > kMxMaxGrid / 4) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul_rows: too large for one launch");
+  hipLaunchKernelGGL((mxfp4_matmul_rows_kernel<BF16, XBF16, NG, WAVES>), dim3((unsigned)grid), dim3(WAVES * 64),
+                     (size_t)(slabs * o.M * 136), s, o.x, o.row_bytes, o.b_codes, o.b_scales, o.c, (int)o.M, o.N, o.K,
+                     (int)slabs, n_units);
+  return check_hip(hipGetLastError(), "smr_mxfp4_matmul_rows launch");
+}
+template <bool BF16, bool XBF16>
+static int launch_rows(const MxRows& o, hipStream_t s) {
+  // Column units and waves per workgroup, K = 8192, us at M = 1 (M = 8):    1 x 8        2 x 16       4 x 8
+  //   N =  3584                                                              5.8  (8.7)   6.4  (8.8)   7.3  (9.9)
+  //   N =  8192                                                              8.3 (11.6)   8.3 (11.0)   9.0 (11.5)
+  //   N = 28672                                                             27.1 (43.0)  27.0 (38.2)  24.7 (29.3)
+  if (o.N <= 4096) return launch_rows_as<BF16, XBF16, 1, 8>(o, s);
+  if (o.N <= 16384) return launch_rows_as<BF16, XBF16, 2, 16>(o, s);
+  return launch_rows_as<BF16, XBF16, 4, 8>(o, s);
+}
+
+template <int BM, int BN>
+static MxTiles tiles_of(const MxOperands& o) {
+  MxTiles t = {o.a_codes, o.a_scales, o.b_codes, o.b_scales, o.c, o.M, o.N};
+  t.slabs = (int)mx_slabs(o.K);
+  t.m_units = (int)mx_row_units(o.M);
+  t.n_units = (int)mx_row_units(o.N);
+  t.tiles_m = (int)((o.M + BM - 1) / BM);
+  t.tiles_n = (int)((o.N + BN - 1) / BN);
+  t.group_m = 8;
+  return t;
+}
+
+// Grids are multiples of 8, so that a workgroup's number says which XCD it is on.
+template <bool BF16, int BM, int BN>
+static int launch_tiles(const MxOperands& o, hipStream_t s) {
+  const MxTiles t = tiles_of<BM, BN>(o);
+  const int64_t total = (int64_t)t.tiles_m * t.tiles_n, cus = compute_units() / 8 * 8;
+  if (total > kMxMaxGrid) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul: too large for one launch");
+  const int64_t grid = total < cus ? (total + 7) / 8 * 8 : cus;
+  hipLaunchKernelGGL((mxfp4_matmul_tile_kernel<BF16, BM, BN>), dim3((unsigned)grid), dim3(kTileThreads), 0, s, t);
+  return check_hip(hipGetLastError(), "smr_mxfp4_matmul launch");
+}
+
+template <bool BF16, int BM, int BN, int BUFFERS>
+static int launch_ring(const MxOperands& o, hipStream_t s) {
+  const MxTiles t = tiles_of<BM, BN>(o);
+  const int64_t total = (int64_t)t.tiles_m * t.tiles_n;
+  if (total > kMxMaxGrid - 8) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul: too large for one launch");
+  hipLaunchKernelGGL((mxfp4_matmul_ring_kernel<BF16, BM, BN, BUFFERS>), dim3((unsigned)((total + 7) / 8 * 8)),
+                     dim3(kTileThreads), 0, s, t);
+  return check_hip(hipGetLastError(), "smr_mxfp4_matmul launch");
+}
+
+// Which kernel: the one with the lowest estimate of its time in microseconds, from launches timed with
+// K = 8192 (32 slabs) on 256 compute units.  A launch costs a few microseconds to start and drain;
+// a slab costs what the busiest compute unit spends on it, by the number of workgroups it gets.
+//                      per slab     M x N with K = 8192, time (us) of few / 64x128 / 128x128 / 256x128 / 256x224
+//   few    64 x 32    0.165-        128x3584:   8.3 /  16 /  20 /  24 /  41
+//   ring   64 x 128   0.41          512x3584:  19.4 /  17 /  21 /  27 /  40
+//   tiles 128 x 128   0.55         1024x3584:  31   /  26 /  22 /  28 /  41
+//   tiles 256 x 128   0.92         2048x3584:  65   /  48 /  41 /  35 /  45
+//   tiles 256 x 224   1.6          4096x3584: 132   /  90 /  84 /  67 /  57
+enum MxKernel { kMxFew, kMxRing64x128, kMxTile128x128, kMxTile256x128, kMxTile256x224 };
+
+static MxKernel pick_kernel(int64_t M, int64_t N, int64_t slabs, int cus) {
+  auto passes = [&](int64_t bm, int64_t bn) { return (double)((((M + bm - 1) / bm) * ((N + bn - 1) / bn) + cus - 1) / cus); };
+  const double n = (double)slabs;
+  const double few_load = (double)((M + 63) / 64) * (double)((N + 31) / 32) / cus * 0.14;
+  const double ring = passes(64, 128);
+  const double time[5] = {3 + n * (few_load > 0.165 ? few_load : 0.165), 4 + n * (ring > 1 ? 0.345 * ring : 0.41),
+                          3 + passes(128, 128) * (2 + 0.55 * n), 3 + passes(256, 128) * (2 + 0.92 * n),
+                          3 + passes(256, 224) * (2 + 1.6 * n)};
+  int best = 0;
+  for (int k = 1; k < 5; ++k)
+    if (time[k] < time[best]) best = k;
+  return (MxKernel)best;
 }
 
 template <bool BF16>
 static int launch_matmul(const MxOperands& o, hipStream_t s) {
-  if (o.M <= 16) return launch_few<BF16, 1, 1, 8>(o, s);
-  return launch_few<BF16, 4, 2, 4>(o, s);
+  // Up to 64 rows B is read once and nothing else counts.  One unit of rows: a unit of columns per
+  // workgroup (N = 8192: 8.0 us, four per workgroup 8.9), four where N alone fills the chip several
+  // times over (N = 28672: 22.4 us, one per workgroup 26).
+  if (o.M <= 16) return o.N <= 16384 ? launch_few<BF16, 1, 1, 8>(o, s) : launch_few<BF16, 1, 4, 8>(o, s);
+  if (o.M <= 32) return launch_few<BF16, 2, 2, 8>(o, s);
+  if (o.M <= 48) return launch_few<BF16, 3, 2, 8>(o, s);
+  if (o.M <= 64) return launch_few<BF16, 4, 2, 8>(o, s);
+  switch (pick_kernel(o.M, o.N, mx_slabs(o.K), compute_units())) {
+    case kMxFew: return launch_few<BF16, 4, 2, 8>(o, s);
+    case kMxRing64x128: return launch_ring<BF16, 64, 128, 3>(o, s);
+    case kMxTile128x128: return launch_tiles<BF16, 128, 128>(o, s);
+    case kMxTile256x128: return launch_tiles<BF16, 256, 128>(o, s);
+    default: return launch_tiles<BF16, 256, 224>(o, s);
+  }
 }
 
 }  // namespace smr
@@ -174,6 +865,37 @@ int smr_mxfp4_matmul(const void* a_codes_dev, const void* a_scales_dev, const vo
                         static_cast<uint8_t*>(c_dev), M, N, K};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return out_dtype == SMR_DTYPE_BF16 ? launch_matmul<true>(o, s) : launch_matmul<false>(o, s);
+}
+
+int64_t smr_mxfp4_matmul_rows_limit(int64_t K) {
+  if (K < 1 || K >= smr::kMxMaxExtent) return SMR_E_INVALID;
+  const int64_t rows = smr::kRowsLdsUnits / smr::mx_slabs(K);
+  return rows < smr::kMxRows ? rows : smr::kMxRows;
+}
+
+int smr_mxfp4_matmul_rows(const void* x_dev, int64_t row_stride, int dtype, const void* b_codes_dev,
+                          const void* b_scales_dev, void* c_dev, int64_t M, int64_t N, int64_t K, int out_dtype,
+                          void* stream) {
+  using namespace smr;
+  if ((dtype != SMR_DTYPE_BF16 && dtype != SMR_DTYPE_FP32) || (out_dtype != SMR_DTYPE_BF16 && out_dtype != SMR_DTYPE_FP32))
+    return fail(SMR_E_INVALID, "smr_mxfp4_matmul_rows: dtype and out_dtype must be bf16 (0) or fp32 (1)");
+  if (M < 0 || N < 0 || K < 1 || N >= kMxMaxExtent || K >= kMxMaxExtent)
+    return fail(SMR_E_INVALID, "smr_mxfp4_matmul_rows: N must be in 0..2^31-1, K in 1..2^31-1");
+  if (M > smr_mxfp4_matmul_rows_limit(K))
+    return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul_rows: more rows than smr_mxfp4_matmul_rows_limit (quantise them first)");
+  if (M > 1 && row_stride < K) return fail(SMR_E_INVALID, "smr_mxfp4_matmul_rows: rows must not overlap (row_stride < K)");
+  if (M == 0 || N == 0) return 0;
+  if (x_dev == nullptr || b_codes_dev == nullptr || b_scales_dev == nullptr || c_dev == nullptr)
+    return fail(SMR_E_INVALID, "smr_mxfp4_matmul_rows: NULL argument");
+  const bool bf16 = dtype == SMR_DTYPE_BF16, out_bf16 = out_dtype == SMR_DTYPE_BF16;
+  if (((reinterpret_cast<uintptr_t>(b_codes_dev) | reinterpret_cast<uintptr_t>(b_scales_dev)) & 15u) ||
+      (reinterpret_cast<uintptr_t>(x_dev) & (bf16 ? 1u : 3u)) || (reinterpret_cast<uintptr_t>(c_dev) & (out_bf16 ? 1u : 3u)))
+    return fail(SMR_E_INVALID, "smr_mxfp4_matmul_rows: misaligned argument (operand: 16 bytes, x and c: one element)");
+  const MxRows o = {static_cast<const uint8_t*>(x_dev), row_stride * (bf16 ? 2 : 4), static_cast<const uint8_t*>(b_codes_dev),
+                    static_cast<const uint8_t*>(b_scales_dev), static_cast<uint8_t*>(c_dev), M, N, K};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (bf16) return out_bf16 ? launch_rows<true, true>(o, s) : launch_rows<false, true>(o, s);
+  return out_bf16 ? launch_rows<true, false>(o, s) : launch_rows<false, false>(o, s);
 }
 
 }  // extern "C"

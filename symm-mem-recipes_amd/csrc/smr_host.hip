@@ -38,6 +38,14 @@ uint64_t* trace_buffer(int64_t min_words) {
   return (p != nullptr && g_trace_words.load(std::memory_order_relaxed) >= min_words) ? p : nullptr;
 }
 
+int compute_units() {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1)
+    return 256;
+  return cus;
+}
+
 uint64_t spin_limit_ticks() {
   int64_t us = g_spin_timeout_us.load(std::memory_order_relaxed);
   return us <= 0 ? 0 : (uint64_t)us * kTicksPerUs;

@@ -16,6 +16,7 @@ void set_last_error(const char* msg);
 int fail(int code, const char* msg);            // records msg, returns code
 int check_hip(hipError_t e, const char* what);  // 0 or the hip error (recorded)
 uint64_t spin_limit_ticks();                    // current timeout in wall_clock64 ticks (0 = none)
+int compute_units();                            // of the current device
 uint64_t* trace_buffer(int64_t min_words);      // the registered trace buffer if it is large enough
 
 // Layout of the optional trace buffer (uint64 words of the 100 MHz device clock):

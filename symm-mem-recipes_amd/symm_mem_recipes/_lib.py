@@ -77,6 +77,8 @@ SIGNATURES = {
     "smr_mxfp4_quantize": (_i, [_p, _i64, _p, _p, _i64, _i64, _i, _i, _p]),
     "smr_mxfp4_dequantize": (_i, [_p, _p, _p, _i64, _i64, _i, _p]),
     "smr_mxfp4_matmul": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p]),
+    "smr_mxfp4_matmul_rows_limit": (_i64, [_i64]),
+    "smr_mxfp4_matmul_rows": (_i, [_p, _i64, _i, _p, _p, _p, _i64, _i64, _i64, _i, _p]),
 }
 
 _lib: Optional[C.CDLL] = None

@@ -25,12 +25,13 @@ BLOCK, UNIT_ROWS, SLAB = 32, 16, 256
 _DTYPE_CODE = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_FP32}
 #: the current stream's handle without building a torch.cuda.Stream object around it
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _call(device: torch.device, what: str, fn, *args) -> None:
     """``fn(*args, stream)`` on ``device``'s current stream, with ``device`` current."""
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -39,15 +40,20 @@ def _call(device: torch.device, what: str, fn, *args) -> None:
         _lib.check(rc, what)
 
 
+def _units(rows: int, cols: int) -> int:
+    return -(-rows // UNIT_ROWS) * -(-cols // SLAB)
+
+
 class MxFp4Tensor:
     """A matrix ``[rows, cols]`` in 4-bit microscaled floats, ``cols`` the axis that a product
     contracts, kept in the order the matrix cores take it (``smr.h``: ``smr_mxfp4_code_bytes``).
-    Made by :func:`mxfp4_quantize` or :meth:`from_blocks`; it owns ``codes`` and ``scales``."""
+    Made by :func:`mxfp4_quantize` or :meth:`from_blocks`; ``storage`` (uint8) holds its codes and,
+    behind them, its scales."""
 
-    __slots__ = ("codes", "scales", "rows", "cols")
+    __slots__ = ("storage", "rows", "cols")
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
-        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+    def __init__(self, storage: torch.Tensor, rows: int, cols: int):
+        self.storage, self.rows, self.cols = storage, rows, cols
 
     @property
     def shape(self) -> torch.Size:
@@ -55,7 +61,19 @@ class MxFp4Tensor:
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self.storage.device
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self.storage[:_units(self.rows, self.cols) * 2048]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self.storage[_units(self.rows, self.cols) * 2048:]
+
+    def _ptrs(self):
+        codes = self.storage.data_ptr()
+        return codes, codes + _units(self.rows, self.cols) * 2048
 
     def __repr__(self) -> str:
         return f"MxFp4Tensor(rows={self.rows}, cols={self.cols}, device={self.device})"
@@ -65,9 +83,7 @@ class MxFp4Tensor:
         """Storage for a matrix, its values undefined."""
         rows, cols = int(rows), int(cols)
         assert 0 <= rows < 2 ** 31 and 1 <= cols < 2 ** 31, "rows must be in 0..2^31-1, cols in 1..2^31-1"
-        units = -(-rows // UNIT_ROWS) * -(-cols // SLAB)
-        return MxFp4Tensor(torch.empty(units * 2048, dtype=torch.uint8, device=device),
-                           torch.empty(units * 128, dtype=torch.uint8, device=device), rows, cols)
+        return MxFp4Tensor(torch.empty(_units(rows, cols) * 2176, dtype=torch.uint8, device=device), rows, cols)
 
     @staticmethod
     def from_blocks(codes: torch.Tensor, scales: torch.Tensor, cols: Optional[int] = None) -> "MxFp4Tensor":
@@ -92,15 +108,15 @@ class MxFp4Tensor:
         exponents = torch.zeros(row_units * UNIT_ROWS, slabs * 8, dtype=torch.uint8, device=codes.device)
         exponents[:rows, :blocks] = scales
         exponents = exponents.view(row_units, UNIT_ROWS, slabs, 2, 4)
-        return MxFp4Tensor(padded.permute(0, 2, 3, 4, 1, 5).contiguous().view(-1),
-                           exponents.permute(0, 2, 4, 1, 3).contiguous().view(-1), rows, cols)
+        return MxFp4Tensor(torch.cat((padded.permute(2, 0, 3, 4, 1, 5).reshape(-1),
+                                      exponents.permute(2, 0, 4, 1, 3).reshape(-1))), rows, cols)
 
     def to_blocks(self):
         """``(codes, scales)`` in the layout :meth:`from_blocks` takes."""
         row_units, slabs = -(-self.rows // UNIT_ROWS), -(-self.cols // SLAB)
         blocks = -(-self.cols // BLOCK)
-        codes = self.codes.view(row_units, slabs, 2, 4, UNIT_ROWS, 16).permute(0, 4, 1, 2, 3, 5)
-        scales = self.scales.view(row_units, slabs, 4, UNIT_ROWS, 2).permute(0, 3, 1, 4, 2)
+        codes = self.codes.view(slabs, row_units, 2, 4, UNIT_ROWS, 16).permute(1, 4, 0, 2, 3, 5)
+        scales = self.scales.view(slabs, row_units, 4, UNIT_ROWS, 2).permute(1, 3, 0, 4, 2)
         return (codes.reshape(row_units * UNIT_ROWS, slabs * SLAB // 2)[:self.rows, :blocks * 16].contiguous(),
                 scales.reshape(row_units * UNIT_ROWS, slabs * 8)[:self.rows, :blocks].contiguous())
 
@@ -108,15 +124,26 @@ class MxFp4Tensor:
         """The values, ``[rows, cols]`` bf16 or fp32 (exact in both)."""
         if out is None:
             assert dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
-            out = torch.empty(self.rows, self.cols, dtype=dtype, device=self.codes.device)
+            out = torch.empty(self.rows, self.cols, dtype=dtype, device=self.storage.device)
         else:
             assert out.dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
             assert tuple(out.shape) == (self.rows, self.cols) and out.is_contiguous(), "out must be contiguous [rows, cols]"
-            assert out.device == self.codes.device, "out must be on the operand's device"
+            assert out.device == self.storage.device, "out must be on the operand's device"
         assert out.is_cuda, "the operand must be on a GPU"
-        _call(out.device, "mxfp4_dequantize", _lib.load().smr_mxfp4_dequantize, self.codes.data_ptr(),
-              self.scales.data_ptr(), out.data_ptr(), self.rows, self.cols, _DTYPE_CODE[out.dtype])
+        _call(out.device, "mxfp4_dequantize", _lib.load().smr_mxfp4_dequantize, *self._ptrs(), out.data_ptr(),
+              self.rows, self.cols, _DTYPE_CODE[out.dtype])
         return out
+
+
+def _check_rows(x: torch.Tensor) -> int:
+    """Validates a matrix whose rows are to be quantised; elements from row to row."""
+    assert x.dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
+    assert x.dim() == 2, "x must be a matrix"
+    rows, cols = x.shape
+    assert cols <= 1 or x.stride(1) == 1, "the elements of a row must be adjacent"
+    row_stride = x.stride(0) if rows > 1 else cols
+    assert row_stride >= cols, "the rows of x must not overlap"
+    return row_stride
 
 
 def mxfp4_quantize(x: torch.Tensor, *, transpose: bool = False, out: Optional[MxFp4Tensor] = None) -> MxFp4Tensor:
@@ -129,21 +156,17 @@ def mxfp4_quantize(x: torch.Tensor, *, transpose: bool = False, out: Optional[Mx
 
     A block's scale is ``2 ** (floor(log2(max |block|)) - 2)``, at least 2^-127; its elements round
     to nearest even and saturate at 6 scales.  A block with an infinity or a NaN becomes NaN."""
-    assert x.dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
-    assert x.dim() == 2, "x must be a matrix"
+    row_stride = _check_rows(x)
     rows, cols = x.shape
-    assert cols <= 1 or x.stride(1) == 1, "the elements of a row must be adjacent"
-    row_stride = x.stride(0) if rows > 1 else cols
-    assert row_stride >= cols, "the rows of x must not overlap"
     shape = (cols, rows) if transpose else (rows, cols)
     assert x.is_cuda, "x must be on a GPU"
     if out is None:
         out = MxFp4Tensor.empty(shape[0], shape[1], x.device)
     else:
         assert (out.rows, out.cols) == shape, "out has another shape"
-        assert out.codes.device == x.device, "out must be on x's device"
+        assert out.device == x.device, "out must be on x's device"
     _call(x.device, "mxfp4_quantize", _lib.load().smr_mxfp4_quantize, x.data_ptr(), row_stride,
-          out.codes.data_ptr(), out.scales.data_ptr(), rows, cols, _DTYPE_CODE[x.dtype], 1 if transpose else 0)
+          *out._ptrs(), rows, cols, _DTYPE_CODE[x.dtype], 1 if transpose else 0)
     return out
 
 
@@ -153,19 +176,29 @@ def mxfp4_matmul(a: Union[MxFp4Tensor, torch.Tensor], b: MxFp4Tensor, *, out_dty
     ``out_dtype`` (bf16 or fp32).  A bf16 or fp32 ``a`` is quantised on the way
     (:func:`mxfp4_quantize`; the result is the same)."""
     assert isinstance(b, MxFp4Tensor), "b must be an MxFp4Tensor"
-    assert len(a.shape) == 2 and a.shape[1] == b.cols, "a and b must be matrices with one contracted extent"
-    device = b.codes.device
+    quantised = isinstance(a, MxFp4Tensor)
+    shape = a.shape
+    assert len(shape) == 2 and shape[1] == b.cols, "a and b must be matrices with one contracted extent"
+    device = b.device
     assert a.device == device, "a and b must be on one device"
     assert device.type == "cuda", "the operands must be on a GPU"
-    if not isinstance(a, MxFp4Tensor):
-        a = mxfp4_quantize(a)
+    M, N = shape[0], b.rows
     if out is None:
         assert out_dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
-        out = torch.empty(a.rows, b.rows, dtype=out_dtype, device=device)
+        out = torch.empty(M, N, dtype=out_dtype, device=device)
     else:
         assert out.dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
-        assert tuple(out.shape) == (a.rows, b.rows) and out.is_contiguous(), "out must be contiguous [M, N]"
+        assert tuple(out.shape) == (M, N) and out.is_contiguous(), "out must be contiguous [M, N]"
         assert out.device == device, "out must be on the operands' device"
-    _call(device, "mxfp4_matmul", _lib.load().smr_mxfp4_matmul, a.codes.data_ptr(), a.scales.data_ptr(),
-          b.codes.data_ptr(), b.scales.data_ptr(), out.data_ptr(), a.rows, b.rows, a.cols, _DTYPE_CODE[out.dtype])
+        out_dtype = out.dtype
+    lib = _lib.load()
+    if not quantised:
+        if M <= UNIT_ROWS and M <= lib.smr_mxfp4_matmul_rows_limit(b.cols):
+            row_stride = _check_rows(a)
+            _call(device, "mxfp4_matmul", lib.smr_mxfp4_matmul_rows, a.data_ptr(), row_stride, _DTYPE_CODE[a.dtype],
+                  *b._ptrs(), out.data_ptr(), M, N, b.cols, _DTYPE_CODE[out_dtype])
+            return out
+        a = mxfp4_quantize(a)
+    _call(device, "mxfp4_matmul", lib.smr_mxfp4_matmul, *a._ptrs(), *b._ptrs(), out.data_ptr(), M, N, b.cols,
+          _DTYPE_CODE[out_dtype])
     return out

@@ -118,7 +118,7 @@ def test_blocks_round_trip_on_the_host(rows, cols):
     want_scales = torch.zeros(-(-rows // 16) * slabs * 128, dtype=torch.uint8)
     for r in range(rows):
         for b in range(blocks):
-            unit, step, lane = (r // 16) * slabs + b // 8, (b % 8) // 4, (b % 4) * 16 + r % 16
+            unit, step, lane = (b // 8) * -(-rows // 16) + r // 16, (b % 8) // 4, (b % 4) * 16 + r % 16
             want_scales[unit * 128 + lane * 2 + step] = scales[r, b]
             for i in range(16):
                 first = b * 32 + 2 * i
