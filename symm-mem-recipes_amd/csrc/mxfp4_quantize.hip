@@ -53,12 +53,6 @@ __global__ __launch_bounds__(kQuantThreads) void mxfp4_quantize_kernel(const uin
   reinterpret_cast<uint16_t*>(scales + unit * kMxScaleBytes)[q * 16 + r] = (uint16_t)mine;
 }
 
-template <bool STREAM, typename T>
-__device__ __forceinline__ T get_any(const T* p) {
-  if constexpr (STREAM) return __builtin_nontemporal_load(p);
-  else return *p;
-}
-
 // Along the columns of x [depth, width]: the result's rows are x's columns, its contracted axis
 // x's rows.  A workgroup takes 64 columns x 256 rows; a thread takes two columns of one block,
 // so a wave reads whole 128-byte lines and a block is one thread's alone.
@@ -79,11 +73,13 @@ __global__ __launch_bounds__(kQuantThreads) void mxfp4_quantize_columns_kernel(
 #pragma unroll
     for (int k = 0; k < 32; ++k) {
       if constexpr (BF16) {
-        const uint32_t w = get_any<STREAM>(reinterpret_cast<const u32_any*>(p + k * row_bytes));
+        const u32_any* at = reinterpret_cast<const u32_any*>(p + k * row_bytes);
+        const uint32_t w = STREAM ? __builtin_nontemporal_load(at) : *at;
         v[0][k] = bf16_lo(w);
         v[1][k] = bf16_hi(w);
       } else {
-        const u32x2 w = get_any<STREAM>(reinterpret_cast<const u32x2_any*>(p + k * row_bytes));
+        const u32x2_any* at = reinterpret_cast<const u32x2_any*>(p + k * row_bytes);
+        const u32x2 w = STREAM ? __builtin_nontemporal_load(at) : *at;
         v[0][k] = __uint_as_float(w.x);
         v[1][k] = __uint_as_float(w.y);
       }
