@@ -399,13 +399,13 @@ int smr_all_reduce_norm(const uint64_t* buffer_ptrs_host, const uint64_t* signal
  * two outputs (grad_residual_out NULL: zero).  grad_partial is the gradient of every rank's
  * partial sums.  Gradients of the weights and of a broadcast gate are summed over what they were
  * broadcast over, in fp32 and in an order that depends on the sizes only.
- *   scratch    smr_norm_backward_scratch_bytes(...) bytes; needs no initialisation */
+ *   scratch    smr_norm_backward_scratch_bytes(...) bytes (NULL where that is 0); needs no initialisation */
 int smr_norm_backward(const void* grad_normed, const void* grad_residual_out, const void* summed,
                       const void* residual_out, const void* weight, const void* post_weight, const void* gate,
                       int gate_kind, void* grad_partial, void* grad_residual, void* grad_weight,
                       void* grad_post_weight, void* grad_gate, float* scratch, int64_t scratch_bytes, int64_t rows,
                       int64_t cols, int dtype, double residual_scale, double eps, void* stream);
-int64_t smr_norm_backward_scratch_bytes(int64_t rows, int64_t cols, int has_post_weight, int gate_kind);
+int64_t smr_norm_backward_scratch_bytes(int64_t rows, int64_t cols, int dtype, int has_post_weight, int gate_kind);
 
 /* 4-bit microscaled operands (OCP MXFP4: e2m1 elements, one e8m0 scale per 32 along the
  * contracted axis), no reference code; the next narrower form of its FP8_OUTPUT switch

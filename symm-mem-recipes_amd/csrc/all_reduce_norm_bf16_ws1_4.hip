@@ -1,0 +1,7 @@
+// bf16 kernels of all_reduce_norm.hpp for world sizes 1 to 4.
+#include "all_reduce_norm.hpp"
+
+SMR_INSTANTIATE_FORWARD(true, 1)
+SMR_INSTANTIATE_FORWARD(true, 2)
+SMR_INSTANTIATE_FORWARD(true, 3)
+SMR_INSTANTIATE_FORWARD(true, 4)

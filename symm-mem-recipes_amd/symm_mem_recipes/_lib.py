@@ -71,7 +71,7 @@ SIGNATURES = {
     "smr_set_gemv_matrix_cores": (_i, [_i]),
     "smr_all_reduce_norm": (_i, [_p, _p, _p, _p, _p, _p, _i, _p, _p, _p, _i64, _i64, _i, _d, _d, _i, _i, _i, _p, _p]),
     "smr_norm_backward": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _d, _d, _p]),
-    "smr_norm_backward_scratch_bytes": (_i64, [_i64, _i64, _i, _i]),
+    "smr_norm_backward_scratch_bytes": (_i64, [_i64, _i64, _i, _i, _i]),
     "smr_mxfp4_code_bytes": (_i64, [_i64, _i64]),
     "smr_mxfp4_scale_bytes": (_i64, [_i64, _i64]),
     "smr_mxfp4_quantize": (_i, [_p, _i64, _p, _p, _i64, _i64, _i, _i, _p]),

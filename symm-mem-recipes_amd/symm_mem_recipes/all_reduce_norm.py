@@ -126,11 +126,11 @@ def one_shot_all_reduce_norm_backward(grad_normed: torch.Tensor, grad_residual_o
                 g.zero_()
         return grads
     lib = _lib.load()
-    scratch = torch.empty(lib.smr_norm_backward_scratch_bytes(rows, cols, post_weight is not None, kind) // 4,
-                          dtype=torch.float32, device=grad_normed.device)
+    dtype = _DTYPE_CODE[grad_normed.dtype]
+    need = lib.smr_norm_backward_scratch_bytes(rows, cols, dtype, post_weight is not None, kind)
+    scratch = torch.empty(need // 4, dtype=torch.float32, device=grad_normed.device) if need else None
     _call(grad_normed.device, "one_shot_all_reduce_norm_backward", lib.smr_norm_backward, grad_normed.data_ptr(),
           _ptr(grad_residual_out), summed.data_ptr(), residual_out.data_ptr(), weight.data_ptr(), _ptr(post_weight),
           _ptr(gate), kind, grads.partial.data_ptr(), grads.residual.data_ptr(), grads.weight.data_ptr(),
-          _ptr(grads.post_weight), _ptr(grads.gate), scratch.data_ptr(), scratch.numel() * 4, rows, cols,
-          _DTYPE_CODE[grad_normed.dtype], float(residual_scale), float(eps))
+          _ptr(grads.post_weight), _ptr(grads.gate), _ptr(scratch), need, rows, cols, dtype, float(residual_scale), float(eps))
     return grads

@@ -58,8 +58,10 @@ def test_norm_argument_errors(lib):
     assert forward() == -1
     assert b"signal pad" in lib.smr_last_error_string()
 
-    need = lib.smr_norm_backward_scratch_bytes(1000, 64, 1, 1)
-    assert need == 3 * 256 * 64 * 4 and lib.smr_norm_backward_scratch_bytes(3, 64, 0, 0) == 3 * 64 * 4
+    need = lib.smr_norm_backward_scratch_bytes(1000, 64, 0, 1, 1)
+    assert need == 3 * 1000 * 64 * 4 and lib.smr_norm_backward_scratch_bytes(1000, 8192, 0, 0, 0) == 256 * 8192 * 4
+    assert lib.smr_norm_backward_scratch_bytes(1, 64, 0, 1, 1) == 0 and lib.smr_norm_backward_scratch_bytes(1000, 3, 1, 1, 1) == 0
+    assert lib.smr_norm_backward_scratch_bytes(1000, 16385, 0, 1, 1) == -1
 
     def backward(dy=p, post=p, gate=p, kind=1, dpost=p, dgate=p, scratch=p, size=need, rows=1000, cols=64):
         return lib.smr_norm_backward(dy, p, p, p, p, post, gate, kind, p, p, p, dpost, dgate, scratch, size, rows, cols, 0, 1.0,
