@@ -12,6 +12,10 @@
 
 #include "all_reduce_norm.hpp"
 
+#define SMR_ELSEWHERE(WS) extern SMR_INSTANTIATE_FORWARD(true, WS) extern SMR_INSTANTIATE_FORWARD(false, WS)
+SMR_ELSEWHERE(1) SMR_ELSEWHERE(2) SMR_ELSEWHERE(3) SMR_ELSEWHERE(4)
+SMR_ELSEWHERE(5) SMR_ELSEWHERE(6) SMR_ELSEWHERE(7) SMR_ELSEWHERE(8)
+
 namespace smr {
 
 int fail_norm(int code, const char* who, const char* what) {

@@ -218,6 +218,7 @@ int launch_forward_ws(const NormForward& f, const SignalPads& pads, int rank, in
 
 }  // namespace smr
 
+// (`extern` in front: in another file)
 #define SMR_INSTANTIATE_FORWARD(BF16, WS)                                                                     \
   template int smr::launch_forward_ws<BF16, WS>(const smr::NormForward&, const smr::SignalPads&, int, int,    \
                                                 uint32_t*, hipStream_t);

@@ -15,20 +15,28 @@ namespace smr {
 struct NormBackward {
   const void *grad_normed, *grad_residual_out, *summed, *residual_out, *weight, *post_weight, *gate;
   void *grad_partial, *grad_residual, *grad_gate;     // grad_gate: kinds token and element only
-  float* sums;                                        // [kinds][gridDim.x][cols]
+  float* sums;                                        // [kinds][parts][cols]
+  float* row_values;                                  // wide rows: r2, r2^2 * mean(dy*weight*h), r1 of each
   void* out[3];                                       // by kind: weight, post_weight, gate (channel)
   int64_t rows;
   int cols, gate_kind;
   float residual_scale, eps;
 };
 
-// AHEAD: the next row's loads are issued before the reductions of the present one.  WHOLE: every vector
-// of every thread is known to lie inside the row.
-template <bool BF16, int CHUNKS, bool AHEAD, bool WHOLE, int THREADS>
+// A row's vectors are loaded AHEAD, before the reductions of the row in front of it, or only KEPT in
+// registers, where two rows would not fit; of rows wider than that they are read again, from the caches,
+// for each phase, and the column sums are another kernel's (norm_columns_kernel).  WHOLE: every vector of
+// every thread is known to lie inside the row.  No variant may spill:
+// builds that kept column sums in scratch memory gave one of them wrong (the ISA test looks for scratch
+// memory).
+enum RowUse { kReread, kKept, kAhead };
+template <bool BF16, int CHUNKS, RowUse USE, bool WHOLE, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward f) {
   using R = Row<BF16>;
   constexpr int V = R::kVec;
-  constexpr bool kKeepWeights = CHUNKS <= 2;
+  constexpr bool kKeep = USE != kReread;
+  constexpr int kHeld = kKeep ? CHUNKS : 1;
+  __shared__ u32x4 weights[2][kKeep ? CHUNKS * THREADS : 1];      // a thread's own vectors of weight and post_weight
   __shared__ float slots3[THREADS / 64][3], slots2[THREADS / 64][2];
   const int waves = blockDim.x >> 6;
   const int cols = f.cols;
@@ -46,138 +54,250 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward f) 
   const void* post_weight = post ? f.post_weight : f.weight;
 
   struct In {
-    u32x4 h[CHUNKS], dy[CHUNKS], s[CHUNKS], dh[CHUNKS], g[CHUNKS];
+    u32x4 h[kHeld], dy[kHeld], s[kHeld], dh[kHeld], g[kHeld];
     float token;
   };
-  auto column = [&](int c) { return (int)(c * blockDim.x + threadIdx.x) * V; };
-  auto load = [&](In& v, int64_t row) __attribute__((always_inline)) {
+  int tid = threadIdx.x;
+  auto column = [&](int c) { return (int)(c * blockDim.x + tid) * V; };
+  auto load_chunk = [&](In& v, int64_t row, int c, int to) __attribute__((always_inline)) {
     const int64_t base = row * row_bytes;
+    v.h[to] = R::template load<kKeep>((const uint8_t*)f.residual_out + base, column(c), cols);
+    v.dy[to] = R::template load<kKeep>((const uint8_t*)f.grad_normed + base, column(c), cols);
+    v.s[to] = R::template load<kKeep>((const uint8_t*)f.summed + base, column(c), cols);
+    v.dh[to] = R::template load<kKeep>(dh_rows + base, column(c), cols);
+    v.g[to] = R::load(gate + row * gate_step, column(c), cols);
+  };
+  auto load = [&](In& v, int64_t row) __attribute__((always_inline)) {
+    if constexpr (kKeep) {
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-      v.h[c] = R::template load<true>((const uint8_t*)f.residual_out + base, column(c), cols);
-      v.dy[c] = R::template load<true>((const uint8_t*)f.grad_normed + base, column(c), cols);
-      v.s[c] = R::template load<true>((const uint8_t*)f.summed + base, column(c), cols);
-      v.dh[c] = R::template load<true>(dh_rows + base, column(c), cols);
-      v.g[c] = R::load(gate + row * gate_step, column(c), cols);
+      for (int c = 0; c < CHUNKS; ++c) load_chunk(v, row, c, c);
     }
     v.token = R::one(token, row * token_step);
   };
   // (the elements of a vector that lies over the row's end belong to the vector before it: its threads
   // compute them too, but count and store only their own)
-  auto own = [&](int c, int e) { return whole || e >= Tail<V>(column(c), cols).shift; };
+  auto first_own = [&](int c) __attribute__((always_inline)) { return whole ? 0 : Tail<V>(column(c), cols).shift; };
   auto put = [&](void* out, int64_t row, int c, float (&v)[V]) __attribute__((always_inline)) {
     if (!whole) Tail<V>(column(c), cols).place(v);
-    R::template store<AHEAD>(static_cast<uint8_t*>(out) + row * row_bytes, column(c), cols, v);
+    R::template store<kKeep>(static_cast<uint8_t*>(out) + row * row_bytes, column(c), cols, v);
   };
 
-  u32x4 w[CHUNKS], p[CHUNKS];
-  if constexpr (kKeepWeights) {
+  if constexpr (kKeep) {
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      w[c] = R::load(f.weight, column(c), cols);
-      p[c] = R::load(post_weight, column(c), cols);
+      weights[0][c * THREADS + threadIdx.x] = R::load(f.weight, column(c), cols);
+      weights[1][c * THREADS + threadIdx.x] = R::load(post_weight, column(c), cols);
     }
   }
-  float sum_w[CHUNKS][V], sum_p[CHUNKS][V], sum_g[CHUNKS][V];
+  // (from LDS: a load from memory would queue up behind the next row's)
+  auto weight_of = [&](int which, int c) __attribute__((always_inline)) {
+    if constexpr (kKeep) return weights[which][c * THREADS + threadIdx.x];
+    else return R::load(which == 0 ? f.weight : post_weight, column(c), cols);
+  };
+  // Column sums of the workgroup's rows.
+  float sum_w[kHeld][V], sum_p[kHeld][V], sum_g[kHeld][V];
 #pragma unroll
-  for (int c = 0; c < CHUNKS; ++c)
+  for (int c = 0; c < kHeld; ++c)
 #pragma unroll
     for (int e = 0; e < V; ++e) sum_w[c][e] = sum_p[c][e] = sum_g[c][e] = 0.0f;
 
   In in;
   float t[3];                                 // sums of h^2, dy*weight*h, s^2
-  auto begin = [&]() __attribute__((always_inline)) {
+  auto begin = [&](int64_t row) __attribute__((always_inline)) {
+    // (recomputed for every row: kept, the addresses of all chunks would take the sums' registers)
+    if constexpr (USE != kAhead) asm volatile("" : "+v"(tid));
     t[0] = t[1] = t[2] = 0.0f;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      if constexpr (!kKeepWeights) w[c] = R::load(f.weight, column(c), cols);
+      const int k = kKeep ? c : 0;
+      if constexpr (!kKeep) load_chunk(in, row, c, 0);
+      const u32x4 w = weight_of(0, c);
+      const int first = first_own(c);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float he = own(c, e) ? R::get(in.h[c], e) : 0.0f, se = own(c, e) ? R::get(in.s[c], e) : 0.0f;
+        const float he = e >= first ? R::get(in.h[k], e) : 0.0f, se = e >= first ? R::get(in.s[k], e) : 0.0f;
         t[0] += he * he;
-        t[1] += R::get(in.dy[c], e) * R::get(w[c], e) * he;
+        t[1] += R::get(in.dy[k], e) * R::get(w, e) * he;
         t[2] += se * se;
+        if constexpr (USE != kAhead)
+          if (e & 1) __builtin_amdgcn_sched_barrier(0);
       }
+      if constexpr (!kKeep) __builtin_amdgcn_sched_barrier(0);
     }
   };
   auto finish = [&](int64_t row) __attribute__((always_inline)) {
+    if constexpr (USE != kAhead) asm volatile("" : "+v"(tid));
     const float token_gate = f.gate_kind == kGateToken ? in.token : 1.0f;
     workgroup_sums<3>(t, slots3, waves);
     const float r2 = 1.0f / sqrtf(t[0] * inv_cols + f.eps);
     const float along = t[1] * inv_cols * r2 * r2;
     const float r1 = post ? 1.0f / sqrtf(t[2] * inv_cols + f.eps) : 1.0f;
-    float d[CHUNKS][V];
+    float d[kKeep ? CHUNKS : 1][V];           // dn*post_weight
     float u[2] = {0.0f, 0.0f};                // sums of dn*post_weight*s and D*n
+    // D of an element
+    auto whole_gradient = [&](int k, int e, const u32x4& w) __attribute__((always_inline)) {
+      const float he = R::get(in.h[k], e), dye = R::get(in.dy[k], e);
+      return (has_dh ? R::get(in.dh[k], e) : 0.0f) + r2 * (dye * R::get(w, e) - he * along);
+    };
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      if constexpr (!kKeepWeights) p[c] = R::load(post_weight, column(c), cols);
-      float out[V], dg[V];
+      const int k = kKeep ? c : 0;
+      if constexpr (!kKeep) load_chunk(in, row, c, 0);
+      const u32x4 w = weight_of(0, c), p = weight_of(1, c);
+      const int first = first_own(c);
+      float out[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float he = R::get(in.h[c], e), se = R::get(in.s[c], e), dye = R::get(in.dy[c], e);
-        const float D = (has_dh ? R::get(in.dh[c], e) : 0.0f) + r2 * (dye * R::get(w[c], e) - he * along);
-        sum_w[c][e] += dye * he * r2;
+        const float D = whole_gradient(k, e, w), se = R::get(in.s[k], e);
         out[e] = f.residual_scale * D;
-        const float pe = post ? R::get(p[c], e) : 1.0f, n = se * r1 * pe;
-        dg[e] = D * n;
-        const float dn = D * (gated ? R::get(in.g[c], e) : token_gate);
-        sum_g[c][e] += dg[e];
-        sum_p[c][e] += dn * se * r1;
-        d[c][e] = dn * pe;
-        if (own(c, e)) {
-          u[0] += d[c][e] * se;
-          u[1] += dg[e];
+        const float pe = post ? R::get(p, e) : 1.0f, dg = D * (se * r1 * pe);
+        const float dn = D * (gated ? R::get(in.g[k], e) : token_gate);
+        if constexpr (kKeep) {
+          sum_w[c][e] += R::get(in.dy[k], e) * R::get(in.h[k], e) * r2;
+          sum_g[c][e] += dg;
+          sum_p[c][e] += dn * se * r1;
         }
+        const float dnp = dn * pe;
+        if constexpr (kKeep) d[c][e] = dnp;
+        u[0] += e >= first ? dnp * se : 0.0f;
+        u[1] += e >= first ? dg : 0.0f;
+        // (a few elements at a time: all of a vector's terms at once would not fit beside the sums)
+        if constexpr (USE != kAhead)
+          if (e & 1) __builtin_amdgcn_sched_barrier(0);
       }
       put(f.grad_residual, row, c, out);
-      if (f.gate_kind == kGateElement) put(f.grad_gate, row, c, dg);
+      if (f.gate_kind == kGateElement) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          out[e] = whole_gradient(k, e, w) * (R::get(in.s[k], e) * r1 * (post ? R::get(p, e) : 1.0f));
+          if constexpr (!kKeep)
+            if (e & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+        put(f.grad_gate, row, c, out);
+      }
+      if constexpr (!kKeep) __builtin_amdgcn_sched_barrier(0);
     }
     workgroup_sums<2>(u, slots2, waves);
     if (f.gate_kind == kGateToken && threadIdx.x == 0) R::put_one(f.grad_gate, row, u[1]);
     const float back = u[0] * inv_cols * r1 * r1;
+    if constexpr (!kKeep)
+      if (threadIdx.x == 0) {
+        f.row_values[row * 3] = r2;
+        f.row_values[row * 3 + 1] = along;
+        f.row_values[row * 3 + 2] = r1;
+      }
+    if constexpr (USE != kAhead) asm volatile("" : "+v"(tid));
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
+      const int k = kKeep ? c : 0;
+      if constexpr (!kKeep) {
+        load_chunk(in, row, c, 0);
+        const u32x4 w = weight_of(0, c), p = weight_of(1, c);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          d[0][e] = whole_gradient(0, e, w) * (gated ? R::get(in.g[0], e) : token_gate) * (post ? R::get(p, e) : 1.0f);
+          if (e & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
 #pragma unroll
       for (int e = 0; e < V; ++e)
-        if (post) d[c][e] = r1 * (d[c][e] - R::get(in.s[c], e) * back);
-      put(f.grad_partial, row, c, d[c]);
+        if (post) d[k][e] = r1 * (d[k][e] - R::get(in.s[k], e) * back);
+      put(f.grad_partial, row, c, d[k]);
+      if constexpr (!kKeep) __builtin_amdgcn_sched_barrier(0);
     }
   };
   int64_t row = blockIdx.x;                   // the grid has no more workgroups than rows
-  load(in, row);
-  for (;;) {
-    begin();
-    const int64_t next = row + gridDim.x;
-    if (next >= f.rows) break;
-    if constexpr (AHEAD) {
+  if constexpr (USE == kAhead) {
+    load(in, row);
+    for (;;) {
+      begin(row);
+      const int64_t next = row + gridDim.x;
+      if (next >= f.rows) break;
       In in_next;
       load(in_next, next);
       finish(row);
       in = in_next;
-    } else {
-      finish(row);
-      load(in, next);
+      row = next;
     }
-    row = next;
+    finish(row);
+  } else {
+    for (; row < f.rows; row += gridDim.x) {
+      load(in, row);
+      begin(row);
+      finish(row);
+    }
   }
-  finish(row);
 
-  auto put_sums = [&](const float (&v)[CHUNKS][V], int kind) {
-    float* out = f.sums + ((int64_t)kind * gridDim.x + blockIdx.x) * cols;
+  if constexpr (kKeep) {
+    auto put_sum = [&](float v, int c, int e, int kind) __attribute__((always_inline)) {
+      const int col = (column(c) < cols - V ? column(c) : cols - V) + e;
+      if (e >= first_own(c)) {
+        if (gridDim.x == 1) R::put_one(f.out[kind], col, v);
+        else f.sums[((int64_t)kind * gridDim.x + blockIdx.x) * cols + col] = v;
+      }
+    };
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const int col = (column(c) < cols - V ? column(c) : cols - V) + e;
-        if (own(c, e)) {
-          if (gridDim.x == 1) R::put_one(f.out[kind], col, v[c][e]);
-          else out[col] = v[c][e];
-        }
+        put_sum(sum_w[c][e], c, e, 0);
+        if (post) put_sum(sum_p[c][e], c, e, 1);
+        if (f.gate_kind == kGateChannel) put_sum(sum_g[c][e], c, e, post ? 2 : 1);
       }
-  };
-  put_sums(sum_w, 0);
-  if (post) put_sums(sum_p, 1);
-  if (f.gate_kind == kGateChannel) put_sums(sum_g, post ? 2 : 1);
+  }
+}
+
+// Column sums for rows whose values norm_backward_kernel left in row_values: a wave takes 64 vectors of
+// columns and every parts-th row; sums as there, [kinds][parts][cols].
+template <bool BF16>
+__global__ __launch_bounds__(64) void norm_columns_kernel(NormBackward f) {
+  using R = Row<BF16>;
+  constexpr int V = R::kVec;
+  const int cols = f.cols, parts = gridDim.y, col = (int)(blockIdx.x * 64 + threadIdx.x) * V;
+  const bool post = f.post_weight != nullptr, has_dh = f.grad_residual_out != nullptr;
+  const bool gated = f.gate_kind == kGateElement || f.gate_kind == kGateChannel;
+  const int64_t row_bytes = (int64_t)cols * R::kSize;
+  const uint8_t* dh_rows = static_cast<const uint8_t*>(has_dh ? f.grad_residual_out : f.residual_out);
+  const uint8_t* gate = static_cast<const uint8_t*>(gated ? f.gate : f.weight);
+  const int64_t gate_step = f.gate_kind == kGateElement ? row_bytes : 0;
+  const void* token = f.gate_kind == kGateToken ? f.gate : f.weight;
+  const int64_t token_step = f.gate_kind == kGateToken ? 1 : 0;
+  const u32x4 w = R::load(f.weight, col, cols), p = R::load(post ? f.post_weight : f.weight, col, cols);
+  float sums[3][V];
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+#pragma unroll
+    for (int e = 0; e < V; ++e) sums[k][e] = 0.0f;
+#pragma unroll 2
+  for (int64_t row = blockIdx.y; row < f.rows; row += parts) {
+    const int64_t base = row * row_bytes;
+    const u32x4 h = R::load((const uint8_t*)f.residual_out + base, col, cols);
+    const u32x4 dy = R::load((const uint8_t*)f.grad_normed + base, col, cols);
+    const u32x4 s = R::load((const uint8_t*)f.summed + base, col, cols);
+    const u32x4 dh = R::load(dh_rows + base, col, cols);
+    const u32x4 g = R::load(gate + row * gate_step, col, cols);
+    const float t = R::one(token, row * token_step), token_gate = f.gate_kind == kGateToken ? t : 1.0f;
+    const float r2 = f.row_values[row * 3], along = f.row_values[row * 3 + 1], r1 = f.row_values[row * 3 + 2];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float he = R::get(h, e), dye = R::get(dy, e), se = R::get(s, e);
+      const float D = (has_dh ? R::get(dh, e) : 0.0f) + r2 * (dye * R::get(w, e) - he * along);
+      sums[0][e] += dye * he * r2;
+      sums[1][e] += D * (gated ? R::get(g, e) : token_gate) * se * r1;
+      sums[2][e] += D * (se * r1 * (post ? R::get(p, e) : 1.0f));
+    }
+  }
+  const int first = Tail<V>(col, cols).shift, at = col < cols - V ? col : cols - V;
+  const int kinds = 1 + post + (f.gate_kind == kGateChannel);
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (e >= first) {
+      float* out = f.sums + (int64_t)blockIdx.y * cols + at + e;
+      const int64_t step = (int64_t)parts * cols;
+      out[0] = sums[0][e];
+      if (post) out[step] = sums[1][e];
+      if (f.gate_kind == kGateChannel) out[(kinds - 1) * step] = sums[2][e];
+    }
 }
 
 // Rows narrower than a vector: one workgroup, a thread per row.
@@ -247,55 +367,64 @@ __global__ __launch_bounds__(256) void norm_backward_narrow_kernel(NormBackward 
 }
 
 // Column sums of the workgroups' contributions: out[kind][col] = sum over parts in an order that depends
-// on their number only.  64 columns per workgroup, 16 threads per column.
+// on their number only.  32 columns (a 128-byte line) per workgroup, 32 threads per column.
 constexpr int kSumThreads = 1024;
 template <bool BF16>
 __global__ __launch_bounds__(kSumThreads) void norm_sums_kernel(const float* __restrict__ sums, int parts, int cols,
                                                                 void* out0, void* out1, void* out2) {
   using R = Row<BF16>;
-  __shared__ float share[16][64];
-  const int col = blockIdx.x * 64 + (threadIdx.x & 63), who = threadIdx.x >> 6;
+  __shared__ float share[32][32];
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31), who = threadIdx.x >> 5;
   void* out = blockIdx.y == 0 ? out0 : (blockIdx.y == 1 ? out1 : out2);
   const float* in = sums + (int64_t)blockIdx.y * parts * cols + (col < cols ? col : cols - 1);
   float t = 0.0f;
   int p = who;
-  for (; p + 7 * 16 < parts; p += 8 * 16) {
+  for (; p + 7 * 32 < parts; p += 8 * 32) {
     float v[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = in[(int64_t)(p + k * 16) * cols];
+    for (int k = 0; k < 8; ++k) v[k] = in[(int64_t)(p + k * 32) * cols];
 #pragma unroll
     for (int k = 0; k < 8; ++k) t += v[k];
   }
-  for (; p < parts; p += 16) t += in[(int64_t)p * cols];
-  share[who][threadIdx.x & 63] = t;
+  for (; p < parts; p += 32) t += in[(int64_t)p * cols];
+  share[who][threadIdx.x & 31] = t;
   __syncthreads();
   if (who == 0 && col < cols) {
 #pragma unroll
-    for (int w = 1; w < 16; ++w) t += share[w][threadIdx.x];
+    for (int w = 1; w < 32; ++w) t += share[w][threadIdx.x];
     R::put_one(out, col, t);
   }
 }
 
-#ifndef DIRECT
-#define DIRECT 5
-#endif
-// How a backward pass is launched; `blocks` > 1 leave cols fp32 sums per kind each.
+// Rows that one workgroup takes, one after the other, instead of one workgroup each and a second launch for
+// their sums: 3 x 4096 8.0 us and 7.8, 5 x 4096 11.0 and 7.7 - but the second launch and its scratch array
+// cost a caller on the host another 4.4 us.
+constexpr int kOneWorkgroupRows = 5;
+
+// How a backward pass is launched; `parts` > 1 leave cols fp32 sums per kind each.
 struct BackwardShape {
-  int threads, chunks, blocks;
-  bool ahead;
+  int threads, chunks, parts;
+  bool wide;                                  // for norm_columns_kernel
 };
 static BackwardShape backward_shape(int64_t rows, int cols, bool bf16) {
-  BackwardShape s = {0, 0, 1, true};
+  BackwardShape s = {0, 0, 1, false};
   const int vec = bf16 ? 8 : 4;
-  if (!norm_shape(cols, vec, 512, s.threads, s.chunks) || s.chunks > 2) {
-    s.ahead = false;                          // wide rows: more threads rather than more registers
+  norm_shape(cols, vec, 512, s.threads, s.chunks);
+  if (s.chunks > 2) {
     norm_shape(cols, vec, 1024, s.threads, s.chunks);
+    // (two chunks of fp32 beside their sums fit 1024 threads' registers, of bf16, twice as many columns, do not)
+    s.wide = bf16 || s.chunks > 2;
   }
-  if (rows > DIRECT) {
+  if (s.wide) {
+    s.parts = (int)(rows < 128 ? rows : 128);
+  } else if (rows > kOneWorkgroupRows) {
     const int64_t most = 256 * (int64_t)(s.threads <= 256 ? 512 / s.threads : 1);
-    s.blocks = (int)(rows < most ? rows : most);
+    s.parts = (int)(rows < most ? rows : most);
   }
   return s;
+}
+static int64_t backward_sums(const BackwardShape& s, int64_t cols, int kinds) {
+  return s.parts == 1 && !s.wide ? 0 : (int64_t)kinds * s.parts * cols;
 }
 
 template <bool BF16>
@@ -307,20 +436,29 @@ static int launch_backward(NormBackward f, hipStream_t s) {
   }
   const BackwardShape b = backward_shape(f.rows, f.cols, BF16);
   const bool whole = f.cols == b.threads * b.chunks * V;
-#define SMR_NORM_LAUNCH(C, AHEAD, WHOLE, T)                                                                            \
-  hipLaunchKernelGGL((norm_backward_kernel<BF16, C, AHEAD, WHOLE, T>), dim3((unsigned)b.blocks), dim3(b.threads), 0, s, f)
-  if (b.ahead && b.chunks == 1 && whole) SMR_NORM_LAUNCH(1, true, true, 512);
-  else if (b.ahead && b.chunks == 1) SMR_NORM_LAUNCH(1, true, false, 512);
-  else if (b.ahead && whole) SMR_NORM_LAUNCH(2, true, true, 512);
-  else if (b.ahead) SMR_NORM_LAUNCH(2, true, false, 512);
-  else if (b.chunks <= 2) SMR_NORM_LAUNCH(2, false, false, 1024);
-  else if constexpr (!BF16) SMR_NORM_LAUNCH(4, false, false, 1024);
+  const int kinds = 1 + (f.out[1] != nullptr) + (f.out[2] != nullptr);
+#define SMR_NORM_LAUNCH(C, USE, WHOLE, T, GRID)                                                                       \
+  hipLaunchKernelGGL((norm_backward_kernel<BF16, C, USE, WHOLE, T>), dim3((unsigned)(GRID)), dim3(b.threads), 0, s, f)
+  if (b.wide) {
+    f.row_values = f.sums + backward_sums(b, f.cols, kinds);
+    const int64_t cus = compute_units(), grid = f.rows < 2 * cus ? f.rows : 2 * cus;
+    if constexpr (BF16) SMR_NORM_LAUNCH(2, kReread, false, 1024, grid);
+    else SMR_NORM_LAUNCH(4, kReread, false, 1024, grid);
+    const int rc = check_hip(hipGetLastError(), "smr_norm_backward launch");
+    if (rc != 0) return rc;
+    hipLaunchKernelGGL((norm_columns_kernel<BF16>), dim3((unsigned)((f.cols + 64 * V - 1) / (64 * V)), (unsigned)b.parts),
+                       dim3(64), 0, s, f);
+  } else if (b.threads > 512) {
+    if constexpr (!BF16) SMR_NORM_LAUNCH(2, kKept, false, 1024, b.parts);
+  } else if (b.chunks == 1 && whole) SMR_NORM_LAUNCH(1, kAhead, true, 512, b.parts);
+  else if (b.chunks == 1) SMR_NORM_LAUNCH(1, kAhead, false, 512, b.parts);
+  else if (whole) SMR_NORM_LAUNCH(2, kAhead, true, 512, b.parts);
+  else SMR_NORM_LAUNCH(2, kAhead, false, 512, b.parts);
 #undef SMR_NORM_LAUNCH
   const int rc = check_hip(hipGetLastError(), "smr_norm_backward launch");
-  if (rc != 0 || b.blocks == 1) return rc;
-  const int kinds = 1 + (f.out[1] != nullptr) + (f.out[2] != nullptr);
-  hipLaunchKernelGGL((norm_sums_kernel<BF16>), dim3((unsigned)((f.cols + 63) / 64), (unsigned)kinds), dim3(kSumThreads), 0,
-                     s, f.sums, b.blocks, f.cols, f.out[0], f.out[1], f.out[2]);
+  if (rc != 0 || (b.parts == 1 && !b.wide)) return rc;
+  hipLaunchKernelGGL((norm_sums_kernel<BF16>), dim3((unsigned)((f.cols + 31) / 32), (unsigned)kinds), dim3(kSumThreads), 0,
+                     s, f.sums, b.parts, f.cols, f.out[0], f.out[1], f.out[2]);
   return check_hip(hipGetLastError(), "smr_norm_backward launch");
 }
 
@@ -334,9 +472,9 @@ int64_t smr_norm_backward_scratch_bytes(int64_t rows, int64_t cols, int dtype, i
     return fail_norm(SMR_E_INVALID, "smr_norm_backward_scratch_bytes", "bad size or dtype");
   const bool bf16 = dtype == SMR_DTYPE_BF16;
   if (cols < (bf16 ? 8 : 4)) return 0;
-  const int blocks = backward_shape(rows, (int)cols, bf16).blocks;
   const int kinds = 1 + (has_post_weight ? 1 : 0) + (gate_kind == kGateChannel ? 1 : 0);
-  return blocks == 1 ? 0 : (int64_t)kinds * blocks * cols * 4;
+  const BackwardShape b = backward_shape(rows, (int)cols, bf16);
+  return (backward_sums(b, cols, kinds) + (b.wide ? rows * 3 : 0)) * 4;
 }
 
 int smr_norm_backward(const void* grad_normed, const void* grad_residual_out, const void* summed,
@@ -368,7 +506,7 @@ int smr_norm_backward(const void* grad_normed, const void* grad_residual_out, co
   NormBackward f = {grad_normed, grad_residual_out, summed, residual_out, weight, post_weight, gate,
                     grad_partial, grad_residual,
                     gate_kind == kGateToken || gate_kind == kGateElement ? grad_gate : nullptr,
-                    scratch, {grad_weight, nullptr, nullptr}, rows, (int)cols, gate_kind, (float)residual_scale, (float)eps};
+                    scratch, nullptr, {grad_weight, nullptr, nullptr}, rows, (int)cols, gate_kind, (float)residual_scale, (float)eps};
   int kinds = 1;
   if (post_weight != nullptr) f.out[kinds++] = grad_post_weight;
   if (gate_kind == kGateChannel) f.out[kinds++] = grad_gate;

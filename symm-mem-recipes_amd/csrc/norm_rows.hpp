@@ -29,7 +29,7 @@ struct Row {
   template <bool STREAM = false>
   static __device__ __forceinline__ u32x4 load(const void* row, int col, int cols) {
     const int at = col < cols - kVec ? col : cols - kVec;
-    GlobalVecAny* p = (GlobalVecAny*)(uintptr_t)(static_cast<const uint8_t*>(row) + (int64_t)at * kSize);
+    GlobalVecAny* p = (GlobalVecAny*)(uintptr_t)(static_cast<const uint8_t*>(row) + (uint32_t)at * (uint32_t)kSize);
     return STREAM ? __builtin_nontemporal_load(p) : *p;
   }
   static __device__ __forceinline__ float get(const u32x4& v, int e) {
@@ -38,7 +38,7 @@ struct Row {
   }
   template <bool STREAM = false>
   static __device__ __forceinline__ void store(void* row, int col, int cols, const float (&f)[kVec]) {
-    uint8_t* p = static_cast<uint8_t*>(row) + (int64_t)col * kSize;
+    uint8_t* p = static_cast<uint8_t*>(row) + (uint32_t)col * (uint32_t)kSize;
     u32x4 v;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -75,6 +75,9 @@ struct Tail {
   __device__ __forceinline__ Tail(int col, int cols) {
     const int over = col - (cols - V);
     shift = over < 0 ? 0 : (over > V ? V : over);
+    // (made anew where it is used: the comparisons with it, kept for every element of every chunk, would
+    // take more scalar registers than there are)
+    asm volatile("" : "+v"(shift));
   }
   // elements to their places, zeros behind the row
   __device__ __forceinline__ void place(float (&f)[V]) const {
@@ -127,7 +130,7 @@ __device__ __forceinline__ void workgroup_sums(float (&v)[N], float (*slots)[N],
 
 // Threads and 128-bit chunks per thread for a row; the smallest number of chunks that fits.
 inline bool norm_shape(int cols, int vec, int max_threads, int& threads, int& chunks) {
-  for (chunks = 1; chunks <= 4; chunks *= 2) {
+  for (chunks = 1; chunks <= 8; chunks *= 2) {
     const int need = (cols + vec * chunks - 1) / (vec * chunks);
     if (need <= max_threads) {
       threads = (need + 63) / 64 * 64;

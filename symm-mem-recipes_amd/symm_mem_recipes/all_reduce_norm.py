@@ -30,19 +30,24 @@ class NormGradients(NamedTuple):
     gate: Optional[torch.Tensor]
 
 
-def _check(like: torch.Tensor, weight, post_weight, gate, same_shape) -> Tuple[int, int, int]:
+def _check(like: torch.Tensor, weight, post_weight, gate, *same_shape) -> Tuple[int, int, int]:
     """Validates the operands of both passes; (rows, cols, gate kind)."""
-    dtype, device, shape = like.dtype, like.device, tuple(like.shape)
+    dtype, device, shape = like.dtype, like.get_device(), like.shape
     assert dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
-    assert like.dim() >= 1 and 1 <= shape[-1] <= MAX_COLS, f"the last dimension must be 1..{MAX_COLS}"
+    assert len(shape) >= 1 and 1 <= shape[-1] <= MAX_COLS, f"the last dimension must be 1..{MAX_COLS}"
     cols = shape[-1]
     rows = like.numel() // cols
-    for t in same_shape:
-        assert tuple(t.shape) == shape, "the tensors must have one shape"
     kind = _GATE_NONE
+    others = [weight, *same_shape]
+    for t in same_shape:
+        assert t.shape == shape, "the tensors must have one shape"
+    assert weight.shape == (cols,), "weights must be [cols]"
+    if post_weight is not None:
+        assert post_weight.shape == (cols,), "weights must be [cols]"
+        others.append(post_weight)
     if gate is not None:
-        gate_shape = tuple(gate.shape)
-        if gate_shape == shape and (len(shape) > 1 or rows != 1):
+        gate_shape = gate.shape
+        if gate_shape == shape and len(shape) > 1:
             kind = _GATE_ELEMENT
         elif gate_shape == (cols,):
             kind = _GATE_CHANNEL
@@ -50,14 +55,13 @@ def _check(like: torch.Tensor, weight, post_weight, gate, same_shape) -> Tuple[i
             kind = _GATE_TOKEN
         else:
             raise AssertionError("gate must be [cols], [..., 1] or of the tensor's shape")
-    for w in (weight, post_weight):
-        assert w is None or tuple(w.shape) == (cols,), "weights must be [cols]"
-    for t in (like, weight, post_weight, gate, *same_shape):
-        if t is not None:
-            assert t.dtype == dtype, "the tensors must have one dtype"
-            assert t.device == device, "the tensors must be on one device"
-            assert t.is_contiguous(), "tensor must be contiguous"
-    assert like.is_cuda, "the tensors must be on a GPU"
+        others.append(gate)
+    assert like.is_contiguous(), "tensor must be contiguous"
+    for t in others:
+        assert t.dtype is dtype, "the tensors must have one dtype"
+        assert t.get_device() == device, "the tensors must be on one device"
+        assert t.is_contiguous(), "tensor must be contiguous"
+    assert device >= 0, "the tensors must be on a GPU"
     return rows, cols, kind
 
 
@@ -88,7 +92,7 @@ def one_shot_all_reduce_norm(tensor: torch.Tensor, residual: torch.Tensor, weigh
     ``barrier``   the blockwise handshake before the peers are read, as one_shot_all_reduce
     ``return_sum`` keep the sum too: the backward pass needs it
     """
-    rows, cols, kind = _check(tensor, weight, post_weight, gate, (residual,))
+    rows, cols, kind = _check(tensor, weight, post_weight, gate, residual)
     if rows == 0:                  # an empty tensor has no address to look up, and there is nothing to reduce
         return tuple(torch.empty_like(tensor) for _ in range(3 if return_sum else 2))
     symm_mem = EmulatedSymmetricMemory.rendezvous(tensor)
@@ -97,7 +101,7 @@ def one_shot_all_reduce_norm(tensor: torch.Tensor, residual: torch.Tensor, weigh
     normed = torch.empty_like(tensor)
     residual_out = torch.empty_like(tensor)
     summed = torch.empty_like(tensor) if return_sum else None
-    _call(tensor.device, "one_shot_all_reduce_norm", _lib.load().smr_all_reduce_norm, symm_mem.buffer_ptrs_host,
+    _call(tensor.get_device(), "one_shot_all_reduce_norm", _lib.load().smr_all_reduce_norm, symm_mem.buffer_ptrs_host,
           symm_mem.signal_pad_ptrs_host if barrier else None, residual.data_ptr(), weight.data_ptr(), _ptr(post_weight),
           _ptr(gate), kind, normed.data_ptr(), residual_out.data_ptr(), _ptr(summed), rows, cols,
           _DTYPE_CODE[tensor.dtype], float(residual_scale), float(eps), symm_mem.rank, symm_mem.world_size,
@@ -116,7 +120,7 @@ def one_shot_all_reduce_norm_backward(grad_normed: torch.Tensor, grad_residual_o
     weights and of a broadcast gate are summed in fp32, in an order that depends on the sizes
     only, and rounded once."""
     same = (summed, residual_out) if grad_residual_out is None else (grad_residual_out, summed, residual_out)
-    rows, cols, kind = _check(grad_normed, weight, post_weight, gate, same)
+    rows, cols, kind = _check(grad_normed, weight, post_weight, gate, *same)
     grads = NormGradients(torch.empty_like(grad_normed), torch.empty_like(grad_normed), torch.empty_like(weight),
                           None if post_weight is None else torch.empty_like(post_weight),
                           None if gate is None else torch.empty_like(gate))
@@ -129,7 +133,7 @@ def one_shot_all_reduce_norm_backward(grad_normed: torch.Tensor, grad_residual_o
     dtype = _DTYPE_CODE[grad_normed.dtype]
     need = lib.smr_norm_backward_scratch_bytes(rows, cols, dtype, post_weight is not None, kind)
     scratch = torch.empty(need // 4, dtype=torch.float32, device=grad_normed.device) if need else None
-    _call(grad_normed.device, "one_shot_all_reduce_norm_backward", lib.smr_norm_backward, grad_normed.data_ptr(),
+    _call(grad_normed.get_device(), "one_shot_all_reduce_norm_backward", lib.smr_norm_backward, grad_normed.data_ptr(),
           _ptr(grad_residual_out), summed.data_ptr(), residual_out.data_ptr(), weight.data_ptr(), _ptr(post_weight),
           _ptr(gate), kind, grads.partial.data_ptr(), grads.residual.data_ptr(), grads.weight.data_ptr(),
           _ptr(grads.post_weight), _ptr(grads.gate), _ptr(scratch), need, rows, cols, dtype, float(residual_scale), float(eps))

@@ -28,9 +28,8 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 
 
-def _call(device: torch.device, what: str, fn, *args) -> None:
-    """``fn(*args, stream)`` on ``device``'s current stream, with ``device`` current."""
-    index = device.index
+def _call(index: int, what: str, fn, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of GPU ``index``, with that GPU current."""
     if index == _current_device():
         rc = fn(*args, _raw_stream(index))
     else:
@@ -81,7 +80,6 @@ class MxFp4Tensor:
     @staticmethod
     def empty(rows: int, cols: int, device) -> "MxFp4Tensor":
         """Storage for a matrix, its values undefined."""
-        rows, cols = int(rows), int(cols)
         assert 0 <= rows < 2 ** 31 and 1 <= cols < 2 ** 31, "rows must be in 0..2^31-1, cols in 1..2^31-1"
         return MxFp4Tensor(torch.empty(_units(rows, cols) * 2176, dtype=torch.uint8, device=device), rows, cols)
 
@@ -122,15 +120,17 @@ class MxFp4Tensor:
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The values, ``[rows, cols]`` bf16 or fp32 (exact in both)."""
+        storage = self.storage
         if out is None:
             assert dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
-            out = torch.empty(self.rows, self.cols, dtype=dtype, device=self.storage.device)
+            out = torch.empty((self.rows, self.cols), dtype=dtype, device=storage.device)
         else:
             assert out.dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
             assert tuple(out.shape) == (self.rows, self.cols) and out.is_contiguous(), "out must be contiguous [rows, cols]"
-            assert out.device == self.storage.device, "out must be on the operand's device"
-        assert out.is_cuda, "the operand must be on a GPU"
-        _call(out.device, "mxfp4_dequantize", _lib.load().smr_mxfp4_dequantize, *self._ptrs(), out.data_ptr(),
+            assert out.device == storage.device, "out must be on the operand's device"
+        assert storage.is_cuda, "the operand must be on a GPU"
+        codes, scales = self._ptrs()
+        _call(storage.get_device(), "mxfp4_dequantize", _lib.load().smr_mxfp4_dequantize, codes, scales, out.data_ptr(),
               self.rows, self.cols, _DTYPE_CODE[out.dtype])
         return out
 
@@ -141,7 +141,9 @@ def _check_rows(x: torch.Tensor) -> int:
     assert x.dim() == 2, "x must be a matrix"
     rows, cols = x.shape
     assert cols <= 1 or x.stride(1) == 1, "the elements of a row must be adjacent"
-    row_stride = x.stride(0) if rows > 1 else cols
+    if rows <= 1:
+        return cols
+    row_stride = x.stride(0)
     assert row_stride >= cols, "the rows of x must not overlap"
     return row_stride
 
@@ -158,15 +160,15 @@ def mxfp4_quantize(x: torch.Tensor, *, transpose: bool = False, out: Optional[Mx
     to nearest even and saturate at 6 scales.  A block with an infinity or a NaN becomes NaN."""
     row_stride = _check_rows(x)
     rows, cols = x.shape
-    shape = (cols, rows) if transpose else (rows, cols)
     assert x.is_cuda, "x must be on a GPU"
     if out is None:
-        out = MxFp4Tensor.empty(shape[0], shape[1], x.device)
+        out = MxFp4Tensor.empty(cols, rows, x.device) if transpose else MxFp4Tensor.empty(rows, cols, x.device)
     else:
-        assert (out.rows, out.cols) == shape, "out has another shape"
+        assert (out.rows, out.cols) == ((cols, rows) if transpose else (rows, cols)), "out has another shape"
         assert out.device == x.device, "out must be on x's device"
-    _call(x.device, "mxfp4_quantize", _lib.load().smr_mxfp4_quantize, x.data_ptr(), row_stride,
-          *out._ptrs(), rows, cols, _DTYPE_CODE[x.dtype], 1 if transpose else 0)
+    codes, scales = out._ptrs()
+    _call(x.get_device(), "mxfp4_quantize", _lib.load().smr_mxfp4_quantize, x.data_ptr(), row_stride, codes, scales, rows,
+          cols, _DTYPE_CODE[x.dtype], 1 if transpose else 0)
     return out
 
 
@@ -195,10 +197,10 @@ def mxfp4_matmul(a: Union[MxFp4Tensor, torch.Tensor], b: MxFp4Tensor, *, out_dty
     if not quantised:
         if M <= UNIT_ROWS and M <= lib.smr_mxfp4_matmul_rows_limit(b.cols):
             row_stride = _check_rows(a)
-            _call(device, "mxfp4_matmul", lib.smr_mxfp4_matmul_rows, a.data_ptr(), row_stride, _DTYPE_CODE[a.dtype],
+            _call(a.get_device(), "mxfp4_matmul", lib.smr_mxfp4_matmul_rows, a.data_ptr(), row_stride, _DTYPE_CODE[a.dtype],
                   *b._ptrs(), out.data_ptr(), M, N, b.cols, _DTYPE_CODE[out_dtype])
             return out
         a = mxfp4_quantize(a)
-    _call(device, "mxfp4_matmul", lib.smr_mxfp4_matmul, *a._ptrs(), *b._ptrs(), out.data_ptr(), M, N, b.cols,
+    _call(device.index, "mxfp4_matmul", lib.smr_mxfp4_matmul, *a._ptrs(), *b._ptrs(), out.data_ptr(), M, N, b.cols,
           _DTYPE_CODE[out_dtype])
     return out
