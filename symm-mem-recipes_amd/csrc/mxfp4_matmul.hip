@@ -33,6 +33,15 @@ __device__ __forceinline__ void put4(uint8_t* p, const f32x4& d) {
     *reinterpret_cast<u32x4_any*>(p) = v;
   }
 }
+// Two fragments of 16 columns side by side: lane group g (16 lanes) holds columns 4g .. 4g+3 of each.  Swapping
+// the odd groups of the first for the even ones of the second gives group g columns 8 (g >> 1) .. +7 of
+// fragment g & 1.
+__device__ __forceinline__ void put8_of_two(uint8_t* p, const f32x4& d0, const f32x4& d1) {
+  const auto lo = __builtin_amdgcn_permlane16_swap(pack_bf16x2(d0[0], d0[1]), pack_bf16x2(d1[0], d1[1]), false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(pack_bf16x2(d0[2], d0[3]), pack_bf16x2(d1[2], d1[3]), false, false);
+  const u32x4 v = {lo[0], hi[0], lo[1], hi[1]};
+  *reinterpret_cast<u32x4_any*>(p) = v;
+}
 // Columns n .. n+3 of row m, as far as they exist.
 template <bool BF16>
 __device__ __forceinline__ void store4(uint8_t* c, int64_t m, int64_t n, int64_t N, const f32x4& d) {
@@ -368,11 +377,19 @@ __device__ __forceinline__ void store_tile(const MxTiles& p, int64_t m0, int64_t
   if (n0 + FN * 16 <= p.N) {
     // all columns exist: one address per row of fragments, the columns are immediate offsets
     uint8_t* out = p.c + (m_lane * p.N + n_lane) * kSize;
+    // bf16: two fragments exchange lane groups, so that a lane has 8 consecutive columns and a row 64 bytes per store
+    const int g = lane >> 4, shift = ((g & 1) * 16 + (g >> 1) * 8 - g * 4) * kSize;
 #pragma unroll
     for (int mi = 0; mi < FM; ++mi) {
       if (m_lane + mi * 16 < p.M) {
+        if constexpr (BF16) {
 #pragma unroll
-        for (int ni = 0; ni < FN; ++ni) put4<BF16>(out + ni * 16 * kSize, acc[ni][mi]);
+          for (int ni = 0; ni + 1 < FN; ni += 2) put8_of_two(out + shift + ni * 16 * kSize, acc[ni][mi], acc[ni + 1][mi]);
+          if constexpr (FN & 1) put4<BF16>(out + (FN - 1) * 16 * kSize, acc[FN - 1][mi]);
+        } else {
+#pragma unroll
+          for (int ni = 0; ni < FN; ++ni) put4<BF16>(out + ni * 16 * kSize, acc[ni][mi]);
+        }
       }
       out += p.N * (16 * kSize);
       __builtin_amdgcn_sched_barrier(0);
