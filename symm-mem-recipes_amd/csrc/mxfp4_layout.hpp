@@ -47,7 +47,6 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t u32_any __attribute__((aligned(2)));
 
-
 // The scale code of a block whose largest |value| has these bits, and the scale as a float.
 __device__ __forceinline__ uint32_t mx_scale_code(uint32_t top_bits) {
   const uint32_t field = top_bits >> 23;

@@ -35,7 +35,8 @@ __device__ __forceinline__ void put4(uint8_t* p, const f32x4& d) {
 }
 // Two fragments of 16 columns side by side: lane group g (16 lanes) holds columns 4g .. 4g+3 of each.  Swapping
 // the odd groups of the first for the even ones of the second gives group g columns 8 (g >> 1) .. +7 of
-// fragment g & 1.
+// fragment g & 1.  (Lanes 16 apart hold the same row: both are there or neither.)  Stores of 32 bytes a row
+// instead of 64: 16384 x 3584 x 8192 224 us, so 214.
 __device__ __forceinline__ void put8_of_two(uint8_t* p, const f32x4& d0, const f32x4& d1) {
   const auto lo = __builtin_amdgcn_permlane16_swap(pack_bf16x2(d0[0], d0[1]), pack_bf16x2(d1[0], d1[1]), false, false);
   const auto hi = __builtin_amdgcn_permlane16_swap(pack_bf16x2(d0[2], d0[3]), pack_bf16x2(d1[2], d1[3]), false, false);
@@ -377,7 +378,6 @@ __device__ __forceinline__ void store_tile(const MxTiles& p, int64_t m0, int64_t
   if (n0 + FN * 16 <= p.N) {
     // all columns exist: one address per row of fragments, the columns are immediate offsets
     uint8_t* out = p.c + (m_lane * p.N + n_lane) * kSize;
-    // bf16: two fragments exchange lane groups, so that a lane has 8 consecutive columns and a row 64 bytes per store
     const int g = lane >> 4, shift = ((g & 1) * 16 + (g >> 1) * 8 - g * 4) * kSize;
 #pragma unroll
     for (int mi = 0; mi < FM; ++mi) {
@@ -814,25 +814,30 @@ static int launch_ring(const MxOperands& o, hipStream_t s) {
   return check_hip(hipGetLastError(), "smr_mxfp4_matmul launch");
 }
 
-// Which kernel: the one with the lowest estimate of its time in microseconds, from launches timed with
-// K = 8192 (32 slabs) on 256 compute units.  A launch costs a few microseconds to start and drain;
-// a slab costs what the busiest compute unit spends on it, by the number of workgroups it gets.
-//                      per slab     M x N with K = 8192, time (us) of few / 64x128 / 128x128 / 256x128 / 256x224
-//   few    64 x 32    0.165-        128x3584:   8.3 /  16 /  20 /  24 /  41
-//   ring   64 x 128   0.41          512x3584:  19.4 /  17 /  21 /  27 /  40
-//   tiles 128 x 128   0.55         1024x3584:  31   /  26 /  22 /  28 /  41
-//   tiles 256 x 128   0.92         2048x3584:  65   /  48 /  41 /  35 /  45
-//   tiles 256 x 224   1.6          4096x3584: 132   /  90 /  84 /  67 /  57
+// Which kernel: the one with the lowest estimate of its time in microseconds, fitted to launches on 256 compute
+// units.  A launch costs a few microseconds to start and drain; a pass of the chip over one tile per compute unit
+// costs its first loads and stores and so much per slab, a pass that is not full at least 0.6 of that; the two kernels
+// without a persistent grid are bound by latency while they fill the chip once.
+//                     n slabs           M x 3584: time (us) of few / 64x128 / 128x128 / 256x128 / 256x224
+//   few    64 x 32    0.75 + 0.117 n     512, K = 8192:  20.5 / 17.5 / 19.8 / 24.6 / 37.3    K = 768:  6.6 /  5.1 /  6.2 /  8.4 / 12.3
+//   ring   64 x 128   1.3  + 0.35  n    1024            33.5 / 25.7 / 22.0 / 27.2 / 38.9             10.9 /  7.2 /  6.9 /  9.0 / 12.8
+//   tiles 128 x 128   2.9  + 0.525 n    2048            66   / 50   / 42   / 34.3 / 45.2             19.0 / 12.0 / 12.0 / 10.7 / 14.4
+//   tiles 256 x 128   6    + 0.78  n    4096           130   / 91   / 81   / 65   / 56               34   / 19.6 / 20.4 / 19.6 / 17
+//   tiles 256 x 224  10.6  + 1.31  n    8192                                                         66   / 35   / 33   / 35   / 31.5
 enum MxKernel { kMxFew, kMxRing64x128, kMxTile128x128, kMxTile256x128, kMxTile256x224 };
 
 static MxKernel pick_kernel(int64_t M, int64_t N, int64_t slabs, int cus) {
-  auto passes = [&](int64_t bm, int64_t bn) { return (double)((((M + bm - 1) / bm) * ((N + bn - 1) / bn) + cus - 1) / cus); };
+  auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+  auto passes = [&](int64_t bm, int64_t bn) {
+    const int64_t all = tiles(bm, bn), rest = all % cus;
+    return (double)(all / cus) + (rest > 0 ? 0.6 + 0.4 * (double)rest / cus : 0.0);
+  };
+  auto larger = [](double a, double b) { return a > b ? a : b; };
   const double n = (double)slabs;
-  const double few_load = (double)((M + 63) / 64) * (double)((N + 31) / 32) / cus * 0.14;
-  const double ring = passes(64, 128);
-  const double time[5] = {3 + n * (few_load > 0.165 ? few_load : 0.165), 4 + n * (ring > 1 ? 0.345 * ring : 0.41),
-                          3 + passes(128, 128) * (2 + 0.55 * n), 3 + passes(256, 128) * (2 + 0.92 * n),
-                          3 + passes(256, 224) * (2 + 1.6 * n)};
+  const double time[5] = {larger(3.3 + 0.157 * n, 3 + (double)tiles(64, 32) / cus * (0.75 + 0.117 * n)),
+                          larger(3.8 + 0.42 * n, 2.5 + passes(64, 128) * (1.3 + 0.35 * n)),
+                          2.4 + passes(128, 128) * (2.9 + 0.525 * n), 3 + passes(256, 128) * (6 + 0.78 * n),
+                          3.5 + passes(256, 224) * (10.6 + 1.31 * n)};
   int best = 0;
   for (int k = 1; k < 5; ++k)
     if (time[k] < time[best]) best = k;

@@ -213,8 +213,9 @@ int smr_mxfp4_quantize(const void* x_dev, int64_t row_stride, void* codes_dev, v
     return fail(SMR_E_INVALID, "smr_mxfp4_quantize: NULL argument");
   const bool bf16 = dtype == SMR_DTYPE_BF16;
   const int64_t size = bf16 ? 2 : 4;
-  if ((reinterpret_cast<uintptr_t>(x_dev) & (size - 1)) || (reinterpret_cast<uintptr_t>(codes_dev) & 15u))
-    return fail(SMR_E_INVALID, "smr_mxfp4_quantize: misaligned argument (codes: 16 bytes, x: one element)");
+  if ((reinterpret_cast<uintptr_t>(x_dev) & (size - 1)) ||
+      ((reinterpret_cast<uintptr_t>(codes_dev) | reinterpret_cast<uintptr_t>(scales_dev)) & 15u))
+    return fail(SMR_E_INVALID, "smr_mxfp4_quantize: misaligned argument (codes and scales: 16 bytes, x: one element)");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream_ptr);
   const uint8_t* x = static_cast<const uint8_t*>(x_dev);
   uint8_t* codes = static_cast<uint8_t*>(codes_dev);
@@ -262,8 +263,9 @@ int smr_mxfp4_dequantize(const void* codes_dev, const void* scales_dev, void* ou
   if (codes_dev == nullptr || scales_dev == nullptr || out_dev == nullptr)
     return fail(SMR_E_INVALID, "smr_mxfp4_dequantize: NULL argument");
   const bool bf16 = dtype == SMR_DTYPE_BF16;
-  if ((reinterpret_cast<uintptr_t>(out_dev) & (bf16 ? 1u : 3u)) || (reinterpret_cast<uintptr_t>(codes_dev) & 15u))
-    return fail(SMR_E_INVALID, "smr_mxfp4_dequantize: misaligned argument (codes: 16 bytes, out: one element)");
+  if ((reinterpret_cast<uintptr_t>(out_dev) & (bf16 ? 1u : 3u)) ||
+      ((reinterpret_cast<uintptr_t>(codes_dev) | reinterpret_cast<uintptr_t>(scales_dev)) & 15u))
+    return fail(SMR_E_INVALID, "smr_mxfp4_dequantize: misaligned argument (codes and scales: 16 bytes, out: one element)");
   const int64_t slabs = mx_slabs(cols), units = mx_row_units(rows) * slabs;
   const int64_t grid = (units + kQuantThreads / 64 - 1) / (kQuantThreads / 64);
   if (grid > kMxMaxGrid) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_dequantize: too large for one launch");

@@ -26,9 +26,8 @@ struct NormBackward {
 // A row's vectors are loaded AHEAD, before the reductions of the row in front of it, or only KEPT in
 // registers, where two rows would not fit; of rows wider than that they are read again, from the caches,
 // for each phase, and the column sums are another kernel's (norm_columns_kernel).  WHOLE: every vector of
-// every thread is known to lie inside the row.  No variant may spill:
-// builds that kept column sums in scratch memory gave one of them wrong (the ISA test looks for scratch
-// memory).
+// every thread is known to lie inside the row.  No variant may spill: builds that kept column sums in
+// scratch memory gave one of them wrong (the ISA test looks for scratch memory).
 enum RowUse { kReread, kKept, kAhead };
 template <bool BF16, int CHUNKS, RowUse USE, bool WHOLE, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward f) {
@@ -115,10 +114,12 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward f) 
       const int first = first_own(c);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float he = e >= first ? R::get(in.h[k], e) : 0.0f, se = e >= first ? R::get(in.s[k], e) : 0.0f;
-        t[0] += he * he;
-        t[1] += R::get(in.dy[k], e) * R::get(w, e) * he;
-        t[2] += se * se;
+        // (the products are masked, not their factors: another vector's infinity must not become a NaN here)
+        const float he = R::get(in.h[k], e), se = R::get(in.s[k], e);
+        const bool own = e >= first;
+        t[0] += own ? he * he : 0.0f;
+        t[1] += own ? R::get(in.dy[k], e) * R::get(w, e) * he : 0.0f;
+        t[2] += own ? se * se : 0.0f;
         if constexpr (USE != kAhead)
           if (e & 1) __builtin_amdgcn_sched_barrier(0);
       }

@@ -17,7 +17,6 @@ enum GateKind : int { kGateNone = 0, kGateChannel = 1, kGateToken = 2, kGateElem
 
 constexpr int kNormMaxCols = 16384;
 
-
 template <bool BF16>
 struct Row {
   static constexpr int kVec = BF16 ? 8 : 4;       // elements of a 128-bit access

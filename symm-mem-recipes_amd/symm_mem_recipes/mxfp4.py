@@ -39,6 +39,23 @@ def _call(index: int, what: str, fn, *args) -> None:
         _lib.check(rc, what)
 
 
+def _span(t: torch.Tensor):
+    """First and last byte + 1 that a tensor's elements lie in."""
+    first = t.data_ptr()
+    return first, first + (1 + sum((n - 1) * step for n, step in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _check_apart(out: torch.Tensor, *inputs: torch.Tensor) -> None:
+    """``out`` shares no memory with ``inputs``: workgroups write while others still read."""
+    if out.numel() == 0:
+        return
+    first, end = _span(out)
+    for t in inputs:
+        if t.numel() != 0:
+            t_first, t_end = _span(t)
+            assert end <= t_first or t_end <= first, "out must not overlap an input"
+
+
 def _units(rows: int, cols: int) -> int:
     return -(-rows // UNIT_ROWS) * -(-cols // SLAB)
 
@@ -52,6 +69,11 @@ class MxFp4Tensor:
     __slots__ = ("storage", "rows", "cols")
 
     def __init__(self, storage: torch.Tensor, rows: int, cols: int):
+        """``storage`` as smr.h lays it out, 16-byte aligned."""
+        assert 0 <= rows < 2 ** 31 and 1 <= cols < 2 ** 31, "rows must be in 0..2^31-1, cols in 1..2^31-1"
+        assert storage.dtype == torch.uint8 and storage.is_contiguous(), "storage must be contiguous uint8"
+        assert storage.shape == (_units(rows, cols) * 2176,), "storage must be [units * 2176]"
+        assert storage.data_ptr() % 16 == 0, "storage must be aligned to 16 bytes"
         self.storage, self.rows, self.cols = storage, rows, cols
 
     @property
@@ -81,7 +103,10 @@ class MxFp4Tensor:
     def empty(rows: int, cols: int, device) -> "MxFp4Tensor":
         """Storage for a matrix, its values undefined."""
         assert 0 <= rows < 2 ** 31 and 1 <= cols < 2 ** 31, "rows must be in 0..2^31-1, cols in 1..2^31-1"
-        return MxFp4Tensor(torch.empty(_units(rows, cols) * 2176, dtype=torch.uint8, device=device), rows, cols)
+        q = MxFp4Tensor.__new__(MxFp4Tensor)
+        q.storage = torch.empty(_units(rows, cols) * 2176, dtype=torch.uint8, device=device)
+        q.rows, q.cols = rows, cols
+        return q
 
     @staticmethod
     def from_blocks(codes: torch.Tensor, scales: torch.Tensor, cols: Optional[int] = None) -> "MxFp4Tensor":
@@ -128,6 +153,7 @@ class MxFp4Tensor:
             assert out.dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
             assert tuple(out.shape) == (self.rows, self.cols) and out.is_contiguous(), "out must be contiguous [rows, cols]"
             assert out.device == storage.device, "out must be on the operand's device"
+            _check_apart(out, storage)
         assert storage.is_cuda, "the operand must be on a GPU"
         codes, scales = self._ptrs()
         _call(storage.get_device(), "mxfp4_dequantize", _lib.load().smr_mxfp4_dequantize, codes, scales, out.data_ptr(),
@@ -154,7 +180,7 @@ def mxfp4_quantize(x: torch.Tensor, *, transpose: bool = False, out: Optional[Mx
 
     ``transpose`` blocks along the columns: the operand of ``x.T``, for products that contract
                   over ``x``'s rows.
-    ``out``       storage of the result's shape to write into.
+    ``out``       an operand of the result's shape to write into, apart from ``x``.
 
     A block's scale is ``2 ** (floor(log2(max |block|)) - 2)``, at least 2^-127; its elements round
     to nearest even and saturate at 6 scales.  A block with an infinity or a NaN becomes NaN."""
@@ -166,6 +192,7 @@ def mxfp4_quantize(x: torch.Tensor, *, transpose: bool = False, out: Optional[Mx
     else:
         assert (out.rows, out.cols) == ((cols, rows) if transpose else (rows, cols)), "out has another shape"
         assert out.device == x.device, "out must be on x's device"
+        _check_apart(out.storage, x)
     codes, scales = out._ptrs()
     _call(x.get_device(), "mxfp4_quantize", _lib.load().smr_mxfp4_quantize, x.data_ptr(), row_stride, codes, scales, rows,
           cols, _DTYPE_CODE[x.dtype], 1 if transpose else 0)
@@ -176,7 +203,7 @@ def mxfp4_matmul(a: Union[MxFp4Tensor, torch.Tensor], b: MxFp4Tensor, *, out_dty
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``a @ b.T`` for ``a`` [M, K] and ``b`` [N, K], accumulated in fp32 and rounded once to
     ``out_dtype`` (bf16 or fp32).  A bf16 or fp32 ``a`` is quantised on the way
-    (:func:`mxfp4_quantize`; the result is the same)."""
+    (:func:`mxfp4_quantize`; the result is the same).  ``out`` may not overlap an operand."""
     assert isinstance(b, MxFp4Tensor), "b must be an MxFp4Tensor"
     quantised = isinstance(a, MxFp4Tensor)
     shape = a.shape
@@ -192,6 +219,7 @@ def mxfp4_matmul(a: Union[MxFp4Tensor, torch.Tensor], b: MxFp4Tensor, *, out_dty
         assert out.dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
         assert tuple(out.shape) == (M, N) and out.is_contiguous(), "out must be contiguous [M, N]"
         assert out.device == device, "out must be on the operands' device"
+        _check_apart(out, a.storage if quantised else a, b.storage)
         out_dtype = out.dtype
     lib = _lib.load()
     if not quantised:

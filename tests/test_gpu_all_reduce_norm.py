@@ -186,6 +186,57 @@ def test_backward(cuda, shape, dtype, post, gate, scale, with_dh):
     assert all(a is None and b is None or torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("shape,dtype", [((3, 1001), "fp32"), ((8, 1003), "bf16"), ((3, 13000), "bf16"), ((2, 64), "bf16"), ((3, 5), "bf16")])
+def test_an_infinite_gradient_stays_an_infinity_whatever_the_width(cuda, shape, dtype):
+    """An infinity near the end of a row, where vectors overlap: its row's gradients are infinite or NaN
+    where the formula's are, its channel's sums too, and the other rows and channels are untouched."""
+    from symm_mem_recipes import one_shot_all_reduce_norm_backward
+    args = _backward_inputs(shape, DTYPES[dtype], True, "channel", True, 3)
+    args[0][1, shape[1] - 2] = float("inf")
+    dy, dh, s, h, w, p, g = _cuda(*args)
+    got = one_shot_all_reduce_norm_backward(dy, dh, s, h, w, post_weight=p, gate=g)
+    want = oracle.backward(*args, 1.0, 1e-6)
+    assert want["residual"][1].isinf().any()
+    for name, b in want.items():
+        a = getattr(got, name).cpu().double()
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.isinf(), b.isinf()), name
+        assert torch.equal(a[a.isinf()].sign(), b[b.isinf()].sign()), name
+    keep = [r for r in range(shape[0]) if r != 1]
+    clean, magnitudes = oracle.backward(*args, 1.0, 1e-6), oracle.backward(*args, 1.0, 1e-6, magnitudes=True)
+    for name in ("residual", "partial"):
+        _within(getattr(got, name)[keep], clean[name][keep], magnitudes[name][keep] * 160 * oracle.U, DTYPES[dtype])
+
+
+def test_offsets_past_32_bits(cuda):
+    """Tensors of more than 4 GiB: the last rows against the oracle, forward and backward."""
+    from symm_mem_recipes import EmulatedSymmetricMemory as SM, one_shot_all_reduce_norm, one_shot_all_reduce_norm_backward
+    for rows, cols in ((270001, 8192), (2200001, 1000), (135001, 16384)):
+        partials, residual, weight, post_weight, g = _inputs((3, cols), 2, torch.bfloat16, True, "element", cols)
+        t = SM.empty_strided_p2p((rows, cols), (cols, 1), torch.bfloat16, "cuda", world_size=2, rank=1)
+        for r in range(2):
+            buf = SM.rendezvous(t).get_buffer(r, (rows, cols), torch.bfloat16)
+            buf.fill_(0.5)
+            buf[-3:] = partials[r].cuda()
+        x, gate = torch.full((rows, cols), 0.25, dtype=torch.bfloat16, device="cuda"), torch.ones(rows, cols, dtype=torch.bfloat16, device="cuda")
+        x[-3:], gate[-3:] = residual.cuda(), g.cuda()
+        w, p = weight.cuda(), post_weight.cuda()
+        y, h, s = one_shot_all_reduce_norm(t, x, w, post_weight=p, gate=gate, return_sum=True)
+        args = (partials, residual, weight, post_weight, g, 1.0, 1e-6)
+        for a, b, c in zip((y, h, s), oracle.forward(*args), oracle.forward_bounds(*args)):
+            _within(a[-3:], b, c, torch.bfloat16)
+        assert torch.equal(y[0], y[-4]) and torch.equal(h[1], h[-5]) and bool((s[:-3] == 1).all())
+        SM.release()
+        del t, buf, x
+        got = one_shot_all_reduce_norm_backward(y, None, s, h, w, post_weight=p, gate=gate)
+        args = (y[-3:].cpu(), None, s[-3:].cpu(), h[-3:].cpu(), weight, post_weight, g, 1.0, 1e-6)
+        want, size = oracle.backward(*args), oracle.backward(*args, magnitudes=True)
+        for name in ("residual", "partial", "gate"):
+            a = getattr(got, name)
+            _within(a[-3:], want[name], size[name] * 160 * oracle.U, torch.bfloat16)
+            assert torch.equal(a[0], a[-4])
+        del y, h, s, gate, got, a
+
+
 def test_backward_against_differences(cuda):
     """Every gradient against central differences of the 64-bit forward pass, through fp32
     inputs: the loss is a weighted sum of both outputs."""

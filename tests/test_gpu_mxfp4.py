@@ -138,6 +138,68 @@ def test_product(cuda, M, N, K, out_dtype):
     assert torch.equal(mxfp4_matmul(qa, qb, out_dtype=out_dtype), got)         # and again
 
 
+# (each of the matrix-tile kernels, one pass over the chip and several; odd widths, units and tiles that end early)
+LARGE = [(300, 3000, 900), (1500, 3500, 1100), (1100, 3001, 700), (2049, 3585, 900), (2000, 3300, 1000), (4097, 3585, 700),
+         (4000, 3584, 1100), (4200, 7201, 1000), (4090, 7161, 1300), (5003, 7392, 257)]
+
+
+@pytest.mark.parametrize("M,N,K", LARGE)
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_large_product(cuda, M, N, K, out_dtype):
+    from symm_mem_recipes import mxfp4_matmul, mxfp4_quantize
+    a, b = _activations(M, K, torch.bfloat16, M + K), _activations(N, K, torch.float32, N + K + 1)
+    qa, qb = mxfp4_quantize(a), mxfp4_quantize(b)
+    room = torch.full((M * N + 512,), 7.0, dtype=out_dtype, device="cuda")
+    got = mxfp4_matmul(qa, qb, out=room[256:256 + M * N].view(M, N))
+    assert bool((room[:256] == 7).all()) and bool((room[256 + M * N:] == 7).all())
+    a64, b64 = (mx.values(*mx.quantize(t))[:, :K].cuda() for t in (a, b))
+    want = a64 @ b64.t()
+    bound = want.abs() * torch.finfo(out_dtype).eps / 2 + (K + 16) * 2.0 ** -24 * (a64.abs() @ b64.abs().t()) * (1 + 2.0 ** -7)
+    off = (got.double() - want).abs()
+    assert bool((off <= bound).all()), float((off - bound).max())
+    for _ in range(2):
+        assert torch.equal(mxfp4_matmul(a, qb, out_dtype=out_dtype), got)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_large_matrices_are_their_parts(cuda, dtype):
+    """Sizes that are streamed past the caches, against the same rows and columns in parts that are not."""
+    from symm_mem_recipes import mxfp4_quantize
+    x = _activations(4101, 8300, torch.bfloat16, 6).to(dtype)
+    whole, columns = mxfp4_quantize(x), mxfp4_quantize(x, transpose=True)
+    codes, scales = whole.to_blocks()
+    t_codes, t_scales = columns.to_blocks()
+    values, t_values = whole.dequantize(dtype), columns.dequantize(dtype)
+    for first in range(0, 4101, 1024):
+        part = mxfp4_quantize(x[first:first + 1024])
+        part_codes, part_scales = part.to_blocks()
+        assert torch.equal(codes[first:first + 1024], part_codes) and torch.equal(scales[first:first + 1024], part_scales)
+        assert torch.equal(values[first:first + 1024], part.dequantize(dtype))
+    for first in range(0, 8300, 2048):
+        part = mxfp4_quantize(x[:, first:first + 2048], transpose=True)
+        part_codes, part_scales = part.to_blocks()
+        assert torch.equal(t_codes[first:first + 2048], part_codes) and torch.equal(t_scales[first:first + 2048], part_scales)
+        assert torch.equal(t_values[first:first + 2048], part.dequantize(dtype))
+
+
+def test_offsets_past_32_bits(cuda):
+    """Inputs, results and storage of more than 4 GiB: the last rows are those of the last rows alone."""
+    from symm_mem_recipes import mxfp4_matmul, mxfp4_quantize
+    tail = _activations(100, 65600, torch.bfloat16, 8)
+    x = torch.zeros(66000, 65600, dtype=torch.bfloat16, device="cuda")         # 8.7 GB, codes 2.2 GB
+    x[-100:] = tail
+    q, part = mxfp4_quantize(x), mxfp4_quantize(tail)
+    assert torch.equal(q.dequantize()[-100:], part.dequantize())
+    del q
+    q, part = mxfp4_quantize(x, transpose=True), mxfp4_quantize(x[:, -64:], transpose=True)
+    assert torch.equal(q.dequantize()[-64:], part.dequantize())
+    del q, x
+    a, b = _activations(70000, 256, torch.bfloat16, 9), mxfp4_quantize(_activations(40001, 256, torch.bfloat16, 10))
+    got = mxfp4_matmul(a, b)                                                   # 5.6 GB
+    assert torch.equal(got[-50:], mxfp4_matmul(a[-50:], b))                    # (one slab: one order of its sum)
+    assert torch.equal(got[34000:34050], mxfp4_matmul(a[34000:34050], b))
+
+
 def test_product_propagates_nan_blocks_to_their_rows_only(cuda):
     from symm_mem_recipes import mxfp4_matmul, mxfp4_quantize
     for M, N in ((5, 40), (200, 300)):
@@ -161,6 +223,24 @@ def test_product_writes_its_result_and_nothing_else(cuda):
             assert mxfp4_matmul(a, b, out=out) is out
             assert bool((room[:128] == 7).all()) and bool((room[128 + M * N:] == 7).all())
             assert torch.equal(out, mxfp4_matmul(a, b, out_dtype=dtype))
+
+
+def test_an_overlapping_result_is_refused(cuda):
+    from symm_mem_recipes import MxFp4Tensor, mxfp4_matmul, mxfp4_quantize
+    x = _activations(4, 64, torch.bfloat16, 0)
+    b = mxfp4_quantize(_activations(64, 64, torch.bfloat16, 1))
+    room = torch.zeros(4 * 64 * 2 + 5 * 2176, dtype=torch.uint8, device="cuda")
+    y = room[:512].view(torch.bfloat16).view(4, 64)
+    with pytest.raises(AssertionError, match="overlap"):
+        mxfp4_matmul(x, b, out=x)
+    with pytest.raises(AssertionError, match="overlap"):
+        mxfp4_matmul(x, b, out=b.storage[:512].view(torch.bfloat16).view(4, 64))
+    with pytest.raises(AssertionError, match="overlap"):
+        mxfp4_quantize(y, out=MxFp4Tensor(room[496:496 + 2176], 4, 64))
+    with pytest.raises(AssertionError, match="overlap"):
+        MxFp4Tensor(room[496:496 + 2176], 4, 64).dequantize(out=y)
+    assert torch.equal(mxfp4_matmul(x, b, out=y), mxfp4_matmul(x, b))           # side by side is apart
+    assert torch.equal(mxfp4_quantize(y, out=MxFp4Tensor(room[512:512 + 2176], 4, 64)).storage, mxfp4_quantize(y).storage)
 
 
 def test_empty_operands(cuda):

@@ -16,12 +16,14 @@ def test_mxfp4_argument_errors(lib):
     assert q(p, 64, None, p, 1, 64, 0, 0, None) == -1
     assert q(p + 1, 64, p, p, 1, 64, 0, 0, None) == -1               # half an element
     assert q(p, 64, p + 8, p, 1, 64, 0, 0, None) == -1               # codes off their boundary
+    assert q(p, 64, p, p + 2, 1, 64, 0, 0, None) == -1
     assert q(p, 2 ** 31 - 1, p, p, 2 ** 31 - 1, 2 ** 31 - 1, 0, 0, None) == -2
     assert q(p, 64, p, p, 0, 64, 0, 0, None) == 0                    # nothing to do: no launch
     d = lib.smr_mxfp4_dequantize
     assert d(p, p, p, 1, 64, 7, None) == -1
     assert d(p, p, None, 1, 64, 0, None) == -1
     assert d(p, p, p + 2, 1, 64, 1, None) == -1                      # fp32 off its boundary
+    assert d(p, p + 8, p, 1, 64, 0, None) == -1
     assert d(p, p, p, 0, 64, 0, None) == 0
     m = lib.smr_mxfp4_matmul
     assert m(p, p, p, p, p, 1, 16, 0, 0, None) == -1                 # nothing contracted
@@ -88,6 +90,13 @@ def test_python_refusals():
         mxfp4_matmul(x, x)
     with pytest.raises(AssertionError):
         b.dequantize()
+    room = torch.zeros(3 * 2176, dtype=torch.uint8)
+    assert MxFp4Tensor(room[16:16 + 2176], 16, 256).shape == (16, 256)
+    for storage, rows, cols in ((room, 16, 256), (room[:2175], 16, 256), (room[8:8 + 2176], 16, 256), (room[::2][:2176], 16, 256),
+                                (room[:2176].view(torch.int8), 16, 256), (room[:2176].view(2, 1088), 16, 256),
+                                (room[:2176], 17, 256), (room[:2176], 16, 257), (room[:0], 0, 0), (room[:0], -1, 256)):
+        with pytest.raises(AssertionError):
+            MxFp4Tensor(storage, rows, cols)
     for codes, scales, cols in (((8, 31), (8, 2), None), ((8, 32), (7, 2), None), ((8, 32), (8, 2), 32), ((8, 32), (8, 2), 65)):
         with pytest.raises(AssertionError):
             MxFp4Tensor.from_blocks(torch.zeros(codes, dtype=torch.uint8), torch.zeros(scales, dtype=torch.uint8), cols)
