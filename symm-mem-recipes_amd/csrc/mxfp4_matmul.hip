@@ -186,8 +186,13 @@ __global__ __launch_bounds__(WAVES * 64) void mxfp4_matmul_rows_kernel(
     const uint8_t* p = x + r * row_bytes + (int64_t)b * 32 * Mx8<XBF16>::kSize;
     const int64_t left = K - (int64_t)b * 32;
     Mx8<XBF16> v[4];
+    if (left >= 32) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j].load(p + j * 8 * Mx8<XBF16>::kSize, left - j * 8);
+      for (int j = 0; j < 4; ++j) v[j].load(p + j * 8 * Mx8<XBF16>::kSize);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j].load(p + j * 8 * Mx8<XBF16>::kSize, left - j * 8);
+    }
     const uint32_t code = mx_scale_code(mx_top<XBF16>(v));
     const float scale = mx_scale_value(code);
     i32x4 w;
@@ -773,9 +778,9 @@ static int launch_rows_as(const MxRows& o, hipStream_t s) {
 template <bool BF16, bool XBF16>
 static int launch_rows(const MxRows& o, hipStream_t s) {
   // Column units and waves per workgroup, K = 8192, us at M = 1 (M = 8):    1 x 8        2 x 16       4 x 8
-  //   N =  3584                                                              5.8  (8.7)   6.4  (8.8)   7.3  (9.9)
-  //   N =  8192                                                              8.3 (11.6)   8.3 (11.0)   9.0 (11.5)
-  //   N = 28672                                                             27.1 (43.0)  27.0 (38.2)  24.7 (29.3)
+  //   N =  3584                                                              5.7  (8.2)   6.3  (8.3)   7.2  (9.6)
+  //   N =  8192                                                              8.3 (11.1)   8.4 (10.5)   8.8 (11.2)
+  //   N = 28672                                                             25.4 (38.4)  26.1 (33.3)  24.4 (27.2)
   if (o.N <= 4096) return launch_rows_as<BF16, XBF16, 1, 8>(o, s);
   if (o.N <= 16384) return launch_rows_as<BF16, XBF16, 2, 16>(o, s);
   return launch_rows_as<BF16, XBF16, 4, 8>(o, s);

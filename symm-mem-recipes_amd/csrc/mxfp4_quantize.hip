@@ -31,21 +31,27 @@ __global__ __launch_bounds__(kQuantThreads) void mxfp4_quantize_kernel(const uin
   const int64_t unit = mx_unit(at / slabs, at % slabs, units / slabs);
   const int r = lane >> 2, q = lane & 3;
   Mx8<BF16> v[8][1];
-  const uint8_t* p = x + (row0 + r) * row_bytes + (col0 + q * 8) * kSize;
-  if (row0 + kMxRows <= rows && col0 + kMxSlab <= cols) {
+  // (rows past the last repeat it and are cleared: loads under a branch would wait for one another)
+  const bool there = row0 + r < rows;
+  const uint8_t* p = x + (there ? row0 + r : rows - 1) * row_bytes + (col0 + q * 8) * kSize;
+  if (col0 + kMxSlab <= cols) {
 #pragma unroll
     for (int b = 0; b < 8; ++b) v[b][0].template load<STREAM>(p + b * 32 * kSize);
   } else {
 #pragma unroll
-    for (int b = 0; b < 8; ++b) v[b][0].load(p + b * 32 * kSize, row0 + r < rows ? cols - col0 - q * 8 - b * 32 : 0);
+    for (int b = 0; b < 8; ++b) v[b][0].load(p + b * 32 * kSize, cols - col0 - q * 8 - b * 32);
   }
+#pragma unroll
+  for (int b = 0; b < 8; ++b)
+#pragma unroll
+    for (uint32_t& w : v[b][0].w) w = there ? w : 0u;
   uint32_t* out = reinterpret_cast<uint32_t*>(codes + unit * kMxCodeBytes) + lane;
   uint32_t mine = 0;              // scales of blocks q and q + 4
 #pragma unroll
   for (int b = 0; b < 8; ++b) {
     uint32_t top = mx_top<BF16>(v[b]);
-    top = max_u32(top, (uint32_t)__shfl_xor((int)top, 1));
-    top = max_u32(top, (uint32_t)__shfl_xor((int)top, 2));
+    top = max_u32(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));   // quad_perm [1,0,3,2]
+    top = max_u32(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));   // quad_perm [2,3,0,1]
     const uint32_t code = mx_scale_code(top);
     out[mx_code_offset(b, 0) / 4] = code == 255u ? 0u : mx_pack8<BF16>(v[b][0], mx_scale_value(code));
     if (q == (b & 3)) mine |= code << (8 * (b >> 2));
@@ -144,13 +150,20 @@ __global__ __launch_bounds__(kQuantThreads) void mxfp4_dequantize_kernel(const u
   if (left <= 0) return;
   const uint8_t* unit_codes = codes + unit * kMxCodeBytes;
   const uint8_t* unit_scales = scales + unit * kMxScaleBytes;
+  // (all rows of a unit are stored, also those behind the matrix: the loads need no branch)
+  uint32_t words[kMxRows / 2], scale_codes[kMxRows / 2];
 #pragma unroll
   for (int i = 0; i < kMxRows / 2; ++i) {
     const int r = i * 2 + (lane >> 5);
-    const int64_t row = row0 + r;
+    words[i] = *reinterpret_cast<const uint32_t*>(unit_codes + mx_code_offset(b, r) + q * 4);
+    scale_codes[i] = unit_scales[mx_scale_offset(b, r)];
+  }
+#pragma unroll
+  for (int i = 0; i < kMxRows / 2; ++i) {
+    const int64_t row = row0 + i * 2 + (lane >> 5);
     if (row >= rows) break;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(unit_codes + mx_code_offset(b, r) + q * 4);
-    const float scale = mx_scale_value(unit_scales[mx_scale_offset(b, r)]);
+    const uint32_t w = words[i];
+    const float scale = mx_scale_value(scale_codes[i]);
     f32x2_t v[4];
     v[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0);
     v[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1);
