@@ -851,14 +851,23 @@ static MxKernel pick_kernel(int64_t M, int64_t N, int64_t slabs, int cus) {
 
 template <bool BF16>
 static int launch_matmul(const MxOperands& o, hipStream_t s) {
-  // Up to 64 rows B is read once and nothing else counts.  One unit of rows: a unit of columns per
-  // workgroup (N = 8192: 8.0 us, four per workgroup 8.9), four where N alone fills the chip several
-  // times over (N = 28672: 22.4 us, one per workgroup 26).
-  if (o.M <= 16) return o.N <= 16384 ? launch_few<BF16, 1, 1, 8>(o, s) : launch_few<BF16, 1, 4, 8>(o, s);
-  if (o.M <= 32) return launch_few<BF16, 2, 2, 8>(o, s);
-  if (o.M <= 48) return launch_few<BF16, 3, 2, 8>(o, s);
-  if (o.M <= 64) return launch_few<BF16, 4, 2, 8>(o, s);
-  switch (pick_kernel(o.M, o.N, mx_slabs(o.K), compute_units())) {
+  // Up to 64 rows B is read once and little else counts.  Times in us, K = 8192, units of columns per workgroup
+  // of the few-rows kernel:
+  //            N = 3584: one / two      8192: one / two       16384: two / ring      28672: two / four / ring
+  //   M = 16   5.2 /                     8.0 /                13.4 / 16.1                    / 24.0 / 22.1
+  //   M = 37   7.0 / 7.3                 9.8 / 8.4
+  //   M = 64   7.3 / 8.3                11.1 / 9.1            14.7 / 16.1             36.9 / 33   / 23.7
+  // Wide products do best with B through LDS, a single unit of rows from K = 2048 on (16 x 131072 x 2048: 28.3 us,
+  // four units 31.7; 16 x 28672 x 1024: 6.1 and 5.4).
+  const int64_t slabs = mx_slabs(o.K);
+  const bool wide = o.N > 16384;
+  if (o.M <= 16 && !wide) return launch_few<BF16, 1, 1, 8>(o, s);
+  if (o.M <= 16 && slabs < 8) return launch_few<BF16, 1, 4, 8>(o, s);
+  if (o.M <= 64 && wide) return launch_ring<BF16, 64, 128, 3>(o, s);
+  if (o.M <= 32) return o.N <= 4096 ? launch_few<BF16, 2, 1, 8>(o, s) : launch_few<BF16, 2, 2, 8>(o, s);
+  if (o.M <= 48) return o.N <= 4096 ? launch_few<BF16, 3, 1, 8>(o, s) : launch_few<BF16, 3, 2, 8>(o, s);
+  if (o.M <= 64) return o.N <= 4096 ? launch_few<BF16, 4, 1, 8>(o, s) : launch_few<BF16, 4, 2, 8>(o, s);
+  switch (pick_kernel(o.M, o.N, slabs, compute_units())) {
     case kMxFew: return launch_few<BF16, 4, 2, 8>(o, s);
     case kMxRing64x128: return launch_ring<BF16, 64, 128, 3>(o, s);
     case kMxTile128x128: return launch_tiles<BF16, 128, 128>(o, s);

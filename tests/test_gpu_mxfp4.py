@@ -122,6 +122,7 @@ PRODUCTS = [
     (1, 1, 1), (1, 16, 32), (1, 256, 8192), (2, 17, 33), (7, 100, 300), (16, 16, 256), (16, 64, 128), (17, 48, 257),
     (31, 3584, 96), (33, 65, 1000), (64, 128, 512), (65, 130, 520), (100, 1001, 77), (128, 128, 4096), (129, 257, 640),
     (256, 224, 256), (257, 225, 768), (300, 449, 1024), (511, 700, 1500), (1000, 333, 2304), (2, 5, 20000),
+    (16, 16401, 300), (5, 16400, 2100), (33, 16395, 520), (64, 17000, 700), (40, 4100, 600), (50, 4500, 300), (20, 4099, 513),
 ]
 
 
