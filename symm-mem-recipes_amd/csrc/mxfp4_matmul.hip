@@ -853,10 +853,10 @@ template <bool BF16>
 static int launch_matmul(const MxOperands& o, hipStream_t s) {
   // Up to 64 rows B is read once and little else counts.  Times in us, K = 8192, units of columns per workgroup
   // of the few-rows kernel:
-  //            N = 3584: one / two      8192: one / two       16384: two / ring      28672: two / four / ring
-  //   M = 16   5.2 /                     8.0 /                13.4 / 16.1                    / 24.0 / 22.1
+  //            N = 3584: one / two      8192: one / two      16384: one / two / ring     28672: two / four / ring
+  //   M = 16   5.2 /                     8.0 /                12.6 /      /                    / 24.0 / 22.1
   //   M = 37   7.0 / 7.3                 9.8 / 8.4
-  //   M = 64   7.3 / 8.3                11.1 / 9.1            14.7 / 16.1             36.9 / 33   / 23.7
+  //   M = 64   7.3 / 8.3                11.1 / 9.1            18.3 / 14.7 / 16.1          36.9 / 33   / 23.7
   // Wide products do best with B through LDS, a single unit of rows from K = 2048 on (16 x 131072 x 2048: 28.3 us,
   // four units 31.7; 16 x 28672 x 1024: 6.1 and 5.4).
   const int64_t slabs = mx_slabs(o.K);

@@ -201,9 +201,10 @@ def mxfp4_quantize(x: torch.Tensor, *, transpose: bool = False, out: Optional[Mx
 
 def mxfp4_matmul(a: Union[MxFp4Tensor, torch.Tensor], b: MxFp4Tensor, *, out_dtype: torch.dtype = torch.bfloat16,
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``a @ b.T`` for ``a`` [M, K] and ``b`` [N, K], accumulated in fp32 and rounded once to
-    ``out_dtype`` (bf16 or fp32).  A bf16 or fp32 ``a`` is quantised on the way
-    (:func:`mxfp4_quantize`; the result is the same).  ``out`` may not overlap an operand."""
+    """``a @ b.T`` for ``a`` [M, K] and ``b`` [N, K], accumulated in fp32 - in an order that depends
+    on the sizes only - and rounded once to ``out_dtype`` (bf16 or fp32).  A bf16 or fp32 ``a`` is
+    quantised on the way, as by :func:`mxfp4_quantize`; for up to 16 rows the order of the sum may
+    then be another.  ``out`` may not overlap an operand."""
     assert isinstance(b, MxFp4Tensor), "b must be an MxFp4Tensor"
     quantised = isinstance(a, MxFp4Tensor)
     shape = a.shape

@@ -101,6 +101,33 @@ def test_the_sum_is_one_shot_all_reduce(cuda):
     SM.release()
 
 
+def test_another_stream_and_a_residual_updated_in_place(cuda, lib):
+    """On a stream of its own, and the C entry with residual_out on top of residual, as it allows: ragged
+    rows, with and without the norm and the handshake that would order the waves."""
+    from symm_mem_recipes import EmulatedSymmetricMemory as SM, one_shot_all_reduce_norm
+    for shape in ((700, 1001), (3, 1001), (600, 2050), (9, 5)):
+        partials, residual, weight, post_weight, _ = _inputs(shape, 4, torch.bfloat16, True, "none", 21)
+        t, handle = _symmetric(partials, 1)
+        x, w, p = _cuda(residual, weight, post_weight)
+        side = torch.cuda.Stream()
+        for pw in (None, p):
+            y, h = one_shot_all_reduce_norm(t, x, w, post_weight=pw)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                y2, h2 = one_shot_all_reduce_norm(t, x, w, post_weight=pw)
+            side.synchronize()
+            assert torch.equal(y, y2) and torch.equal(h, h2)
+            for mode in (0, 1):
+                x2, y3 = x.clone(), torch.empty_like(y)
+                rc = lib.smr_all_reduce_norm(handle.buffer_ptrs_host, handle.signal_pad_ptrs_host, x2.data_ptr(), w.data_ptr(),
+                                             0 if pw is None else pw.data_ptr(), None, 0, y3.data_ptr(), x2.data_ptr(), None,
+                                             shape[0], shape[1], 0, 1.0, 1e-6, 1, 4, mode, handle.status.data_ptr(),
+                                             torch.cuda.current_stream().cuda_stream)
+                assert rc == 0 and torch.equal(x2, h) and torch.equal(y3, y)
+        handle.check_status()
+    SM.release()
+
+
 def test_rows_of_zeros_infinities_and_nan(cuda):
     """A row of zeros divides by sqrt(eps) and stays zero; an infinity or NaN spoils its own row
     and no other."""
