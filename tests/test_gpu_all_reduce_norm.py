@@ -62,6 +62,11 @@ FORWARD = [
     ((2, 8200), 8, "bf16", True, "element", 1.0), ((2, 16384), 4, "bf16", True, "none", 1.0),
     ((2, 16383), 3, "bf16", True, "token", 1.0), ((2, 16381), 2, "fp32", True, "channel", 1.0),
     ((1030, 2048), 6, "bf16", True, "token", 1.0), ((5000, 40), 8, "fp32", True, "element", 1.0),
+    # more rows than compute units, wide enough that a workgroup loads its next row ahead
+    ((300, 8192), 8, "bf16", True, "channel", 1.0), ((530, 8001), 7, "bf16", False, "element", 1.0), ((260, 4096), 1, "bf16", True, "token", 0.5),
+    ((777, 2999), 5, "bf16", True, "none", 1.0), ((270, 4096), 4, "fp32", False, "token", 1.0), ((300, 4093), 3, "fp32", True, "element", 1.0),
+    ((513, 2048), 6, "fp32", False, "none", 1.0), ((300, 1025), 2, "fp32", True, "channel", 1.0), ((4200, 1100), 2, "bf16", True, "element", 1.0),
+    ((300, 9000), 3, "bf16", True, "channel", 1.0), ((300, 9001), 2, "fp32", False, "element", 1.0),
 ]
 
 
@@ -181,6 +186,13 @@ BACKWARD = [
     ((2, 8200), "bf16", True, "element", 1.0, True), ((2, 16384), "bf16", True, "channel", 1.0, True),
     ((2, 16383), "bf16", True, "token", 1.0, True), ((2, 16381), "fp32", True, "channel", 1.0, True),
     ((1030, 2048), "bf16", True, "token", 1.0, True), ((5000, 40), "fp32", True, "element", 1.0, True),
+    # several rows per workgroup: rows ahead of one and of two vectors a thread, rows kept, rows read again
+    ((600, 4096), "bf16", False, "channel", 1.0, False), ((520, 8192), "bf16", True, "channel", 1.0, True),
+    ((530, 8001), "bf16", True, "element", 1.0, True), ((513, 2999), "bf16", True, "none", -1.0, True),
+    ((260, 4096), "fp32", True, "token", 1.0, True), ((300, 4093), "fp32", True, "channel", 1.0, False),
+    ((270, 8192), "fp32", True, "channel", 1.0, True), ((265, 8191), "fp32", False, "element", 1.0, True),
+    ((300, 9001), "fp32", True, "channel", 1.0, True), ((300, 16384), "bf16", True, "token", 1.0, False),
+    ((520, 8201), "bf16", True, "channel", 1.0, True),
 ]
 
 
@@ -195,7 +207,7 @@ def _backward_inputs(shape, dtype, post, gate, with_dh, seed):
 def test_backward(cuda, shape, dtype, post, gate, scale, with_dh):
     """Every term of a gradient passes through at most 128 roundings on its way (32 values and 22
     partial sums in each of two row sums, the rest single operations); a column sum adds at most
-    rows / 256 terms in a workgroup, 16 of each thread's and 16 threads'."""
+    rows / 128 terms in a workgroup, 32 workgroups' in a thread and 32 threads'."""
     from symm_mem_recipes import one_shot_all_reduce_norm_backward
     dtype = DTYPES[dtype]
     args = _backward_inputs(shape, dtype, post, gate, with_dh, sum(shape))
@@ -207,7 +219,7 @@ def test_backward(cuda, shape, dtype, post, gate, scale, with_dh):
     rows = dy.numel() // dy.shape[-1]
     for name, b in want.items():
         a = getattr(got, name)
-        off = size[name] * (128 + rows / 256 + 32) * oracle.U
+        off = size[name] * (128 + rows / 128 + 64) * oracle.U
         _within(a.reshape(b.shape), b, off, dtype)
     again = one_shot_all_reduce_norm_backward(dy, dh, s, h, w, post_weight=p, gate=g, residual_scale=scale, eps=1e-5)
     assert all(a is None and b is None or torch.equal(a, b) for a, b in zip(got, again))

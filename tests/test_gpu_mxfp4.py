@@ -52,6 +52,31 @@ def test_quantize_takes_rows_that_are_apart_and_any_alignment(cuda, dtype, trans
         _same_operand(mxfp4_quantize(x, transpose=transpose), *mx.quantize(x.t() if transpose else x))
 
 
+@pytest.mark.parametrize("rows,cols", [(3, 40), (17, 257), (70, 1001)])
+def test_storage_is_written_whole(cuda, rows, cols):
+    """A used operand written over holds nothing of what it was, in its padding either."""
+    from symm_mem_recipes import MxFp4Tensor, mxfp4_quantize
+    x = _activations(rows, cols, torch.bfloat16, 12)
+    for transpose in (False, True):
+        fresh = mxfp4_quantize(x, transpose=transpose)
+        used = MxFp4Tensor(torch.full_like(fresh.storage, 255), fresh.rows, fresh.cols)
+        assert mxfp4_quantize(x, transpose=transpose, out=used) is used
+        assert torch.equal(used.storage, fresh.storage)
+        assert torch.equal(MxFp4Tensor.from_blocks(*fresh.to_blocks(), fresh.cols).storage, fresh.storage)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_product_of_rows_that_are_apart_and_any_alignment(cuda, dtype):
+    from symm_mem_recipes import mxfp4_matmul, mxfp4_quantize
+    whole = _activations(60, 700, dtype, 14)
+    for a in (whole[:16, 1:600], whole[5:6, 3:], whole[::7, 2:34], whole[:, 1:402], whole[3:20, :31]):
+        K = a.shape[1]
+        b = mxfp4_quantize(_activations(50, K, torch.bfloat16, K))
+        assert torch.equal(mxfp4_matmul(a, b), mxfp4_matmul(a.contiguous(), b))
+        _check_product(mxfp4_matmul(a, b), mx.values(*mx.quantize(a))[:, :K],
+                       b.dequantize(torch.float32).cpu().double(), torch.bfloat16)
+
+
 def test_quantize_special_values(cuda):
     """Every rounding border and its neighbours, both signs, at scales up to the ends of the
     range; zeros, subnormals, the largest value, infinities and NaN."""
