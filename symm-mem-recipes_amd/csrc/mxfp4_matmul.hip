@@ -625,8 +625,11 @@ __global__ __launch_bounds__(kTileThreads, 1) void mxfp4_matmul_tile_kernel(MxTi
 
 // ---------------------------------------------------------------------------
 // The same product in smaller tiles, for results that have too few of the large ones to fill the
-// chip.  What bounds those is the time a slab takes to arrive, so LDS holds BUFFERS whole slab pairs
-// and all but the two being multiplied and read are on their way; the order inside a pair is the compiler's.
+// chip.  What bounds those is the arrival of the slabs - first the latency, then the 62 bytes/ns that a compute
+// unit receives (64 x 128: 26 KB per slab pair in 0.42 us) - so LDS holds BUFFERS whole slab pairs and all but the
+// two being multiplied and read are on their way; the order inside a pair is the compiler's.  Three: two workgroups
+// fit a compute unit (1500 x 3500 x 1100: 11.9 us, with four 14.6), and alone four to six are no faster (1001 x
+// 1777 x 4000: 11.8, 12.0, 12.3, 12.4), nor is a second group of waves that takes every other slab (12.2).
 // One tile per workgroup.
 template <bool BF16, int BM, int BN, int BUFFERS>
 __global__ __launch_bounds__(kTileThreads) void mxfp4_matmul_ring_kernel(MxTiles p) {

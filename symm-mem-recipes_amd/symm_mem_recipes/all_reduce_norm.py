@@ -2,7 +2,7 @@
 behind the block, its gate, the scaled residual and the norm in front of the next block; and
 the backward pass.  The reference stops at the reduce
 (symm_mem_recipes/triton_one_shot_all_reduce.py:96-125); validation, handshake and ownership
-are ``one_shot_all_reduce``'s.
+are ``one_shot_all_reduce``'s.  Nothing here is recorded by autograd.
 """
 from __future__ import annotations
 
@@ -89,7 +89,8 @@ def one_shot_all_reduce_norm(tensor: torch.Tensor, residual: torch.Tensor, weigh
     ``weight``, ``post_weight``  [cols]
     ``gate``      [cols] (one per channel), [..., 1] (one per token) or of ``tensor``'s shape; a
                   one-dimensional gate of a one-dimensional tensor is per channel
-    ``barrier``   the blockwise handshake before the peers are read, as one_shot_all_reduce
+    ``barrier``   the blockwise handshake before the peers are read, as one_shot_all_reduce, and on the
+                  same signal pads: calls on one allocation belong on one stream at a time
     ``return_sum`` keep the sum too: the backward pass needs it
     """
     rows, cols, kind = _check(tensor, weight, post_weight, gate, residual)

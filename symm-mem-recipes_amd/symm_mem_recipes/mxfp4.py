@@ -10,6 +10,8 @@ outputs and over the tokens; ``mxfp4_quantize(..., transpose=True)`` gives their
     dx = mxfp4_matmul(dy, mxfp4_quantize(w, transpose=True))      # contracts over N
     dw = mxfp4_matmul(mxfp4_quantize(dy, transpose=True),         # contracts over T
                       mxfp4_quantize(x, transpose=True))
+
+Nothing here is recorded by autograd.
 """
 from __future__ import annotations
 
