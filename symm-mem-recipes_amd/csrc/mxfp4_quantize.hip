@@ -17,49 +17,60 @@ namespace smr {
 
 constexpr int kQuantThreads = 256;
 
-// Along the rows of x.  A wave takes one unit; lane 4 r + q holds quarter q of a block of row r, the
-// eight blocks of the slab in turn: the codes of a block of all 16 rows are 256 contiguous bytes, and
-// so is a store.  Four lanes that share a block find its scale, and between them hold the scales of the
-// row's eight blocks.
+// Along the rows of x.  A wave takes one unit, 8 elements of a block per lane and load; four lanes that share
+// a block find its scale, and between them hold the scales of their rows' eight blocks.  A load takes one
+// block of all 16 rows, and their codes are 256 contiguous bytes - or, from memory (STREAM), two blocks of 8
+// rows, whole lines of bf16 (16384 x 8192 55 us, block by block 60; 16384 x 8200 63 and 74; out of the caches
+// 1001 x 4000 4.5 and 4.3, fp32 6.6 and 6.1).
 template <bool BF16, bool STREAM>
 __global__ __launch_bounds__(kQuantThreads) void mxfp4_quantize_kernel(const uint8_t* __restrict__ x, int64_t row_bytes,
                                                                       uint8_t* __restrict__ codes,
                                                                       uint8_t* __restrict__ scales, int64_t rows,
                                                                       int64_t cols, int64_t slabs, int64_t units) {
   constexpr int kSize = BF16 ? 2 : 4;
+  constexpr int kWide = STREAM ? 2 : 1;                       // blocks per load
+  constexpr int kRows = kMxRows / kWide, kSteps = 8 / kWide;  // rows per load, loads per row
   const int lane = threadIdx.x & 63;
   const int64_t at = (int64_t)blockIdx.x * (kQuantThreads / 64) + (threadIdx.x >> 6);
   if (at >= units) return;
   const int64_t row0 = at / slabs * kMxRows, col0 = at % slabs * kMxSlab;
   const int64_t unit = mx_unit(at / slabs, at % slabs, units / slabs);
-  const int r = lane >> 2, q = lane & 3;
-  Mx8<BF16> v[8][1];
-  // (rows past the last repeat it and are cleared: loads under a branch would wait for one another)
-  const bool there = row0 + r < rows;
-  const uint8_t* p = x + (there ? row0 + r : rows - 1) * row_bytes + (col0 + q * 8) * kSize;
-  if (col0 + kMxSlab <= cols) {
+  const int r = lane / (4 * kWide), side = (lane >> 2) % kWide, q = lane & 3;
+  const int64_t col = col0 + side * 32 + q * 8;
+  Mx8<BF16> v[kWide][kSteps][1];
 #pragma unroll
-    for (int b = 0; b < 8; ++b) v[b][0].template load<STREAM>(p + b * 32 * kSize);
-  } else {
+  for (int i = 0; i < kWide; ++i) {
+    // (rows past the last repeat it and are cleared: loads under a branch would wait for one another)
+    const int64_t row = row0 + i * kRows + r;
+    const uint8_t* p = x + (row < rows ? row : rows - 1) * row_bytes + col * kSize;
+    if (col0 + kMxSlab <= cols) {
 #pragma unroll
-    for (int b = 0; b < 8; ++b) v[b][0].load(p + b * 32 * kSize, cols - col0 - q * 8 - b * 32);
+      for (int j = 0; j < kSteps; ++j) v[i][j][0].template load<STREAM>(p + j * (kWide * 32 * kSize));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) v[i][j][0].load(p + j * (kWide * 32 * kSize), cols - col - j * (kWide * 32));
+    }
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+      for (uint32_t& w : v[i][j][0].w) w = row < rows ? w : 0u;
   }
+  uint32_t* out = reinterpret_cast<uint32_t*>(codes + unit * kMxCodeBytes) + q;
+  uint32_t mine = 0;              // scales of a block and the fourth after it, of one of the lane's rows
 #pragma unroll
-  for (int b = 0; b < 8; ++b)
+  for (int i = 0; i < kWide; ++i)
 #pragma unroll
-    for (uint32_t& w : v[b][0].w) w = there ? w : 0u;
-  uint32_t* out = reinterpret_cast<uint32_t*>(codes + unit * kMxCodeBytes) + lane;
-  uint32_t mine = 0;              // scales of blocks q and q + 4
-#pragma unroll
-  for (int b = 0; b < 8; ++b) {
-    uint32_t top = mx_top<BF16>(v[b]);
-    top = max_u32(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));   // quad_perm [1,0,3,2]
-    top = max_u32(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));   // quad_perm [2,3,0,1]
-    const uint32_t code = mx_scale_code(top);
-    out[mx_code_offset(b, 0) / 4] = code == 255u ? 0u : mx_pack8<BF16>(v[b][0], mx_scale_value(code));
-    if (q == (b & 3)) mine |= code << (8 * (b >> 2));
-  }
-  reinterpret_cast<uint16_t*>(scales + unit * kMxScaleBytes)[q * 16 + r] = (uint16_t)mine;
+    for (int j = 0; j < kSteps; ++j) {
+      uint32_t top = mx_top<BF16>(v[i][j]);
+      top = max_u32(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));   // quad_perm [1,0,3,2]
+      top = max_u32(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));   // quad_perm [2,3,0,1]
+      const uint32_t code = mx_scale_code(top);
+      out[mx_code_offset(j * kWide + side, i * kRows + r) / 4] =
+          code == 255u ? 0u : mx_pack8<BF16>(v[i][j][0], mx_scale_value(code));
+      if (q == i * (kSteps / 2) + j % (kSteps / 2)) mine |= code << (8 * (j / (kSteps / 2)));
+    }
+  const int of_row = q / (kSteps / 2) * kRows + r, of_block = q % (kSteps / 2) * kWide + side;
+  reinterpret_cast<uint16_t*>(scales + unit * kMxScaleBytes)[of_block * 16 + of_row] = (uint16_t)mine;
 }
 
 // Along the columns of x [depth, width]: the result's rows are x's columns, its contracted axis
@@ -237,7 +248,7 @@ int smr_mxfp4_quantize(const void* x_dev, int64_t row_stride, void* codes_dev, v
   uint8_t* codes = static_cast<uint8_t*>(codes_dev);
   uint8_t* scales = static_cast<uint8_t*>(scales_dev);
   // Past the caches from 64 MiB on: what the caches can hold may be there (4096 x 4096 bf16 9.3 us, streamed
-  // 10.0), what they cannot only drives the codes out of them (16384 x 8192 64 us, streamed 60; along
+  // 10.0), what they cannot only drives the codes out of them (16384 x 8192 64 us, streamed 55; along
   // the columns 75 and 65; with the codes read back behind it 164 and 133).
   const bool stream = rows * cols * size >= ((int64_t)64 << 20);
   if (transpose) {
