@@ -9,8 +9,8 @@
 // (v_cvt_scalef32_pk_fp4_f32: the scale is a power of two, so the division is exact and there is
 // one rounding).
 //
-// All of it is bound by memory: 16384 x 8192 bf16 59 us (340 MB, 5.7 TB/s) and back 50 us, 8191 x 3584 fp32 along
-// the columns 28 us (4.75 TB/s); a single row takes a launch and two trips to memory, 3.3 us.
+// All of it is bound by memory: 16384 x 8192 bf16 55 us (340 MB, 6.2 TB/s) and back 50 us, 8191 x 3584 fp32 along
+// the columns 26.6 us (5.0 TB/s); a single row takes a launch and two trips to memory, 3.3 us.
 #include "mxfp4_layout.hpp"
 
 namespace smr {
@@ -26,15 +26,16 @@ template <bool BF16, bool STREAM>
 __global__ __launch_bounds__(kQuantThreads) void mxfp4_quantize_kernel(const uint8_t* __restrict__ x, int64_t row_bytes,
                                                                       uint8_t* __restrict__ codes,
                                                                       uint8_t* __restrict__ scales, int64_t rows,
-                                                                      int64_t cols, int64_t slabs, int64_t units) {
+                                                                      int64_t cols, uint32_t slabs, uint32_t units) {
   constexpr int kSize = BF16 ? 2 : 4;
   constexpr int kWide = STREAM ? 2 : 1;                       // blocks per load
   constexpr int kRows = kMxRows / kWide, kSteps = 8 / kWide;  // rows per load, loads per row
   const int lane = threadIdx.x & 63;
-  const int64_t at = (int64_t)blockIdx.x * (kQuantThreads / 64) + (threadIdx.x >> 6);
+  const uint32_t at = blockIdx.x * (kQuantThreads / 64) + (threadIdx.x >> 6);
   if (at >= units) return;
-  const int64_t row0 = at / slabs * kMxRows, col0 = at % slabs * kMxSlab;
-  const int64_t unit = mx_unit(at / slabs, at % slabs, units / slabs);
+  const uint32_t row_unit = at / slabs, slab = at - row_unit * slabs;
+  const int64_t row0 = (int64_t)row_unit * kMxRows, col0 = (int64_t)slab * kMxSlab;
+  const int64_t unit = mx_unit(row_unit, slab, units / slabs);
   const int r = lane / (4 * kWide), side = (lane >> 2) % kWide, q = lane & 3;
   const int64_t col = col0 + side * 32 + q * 8;
   Mx8<BF16> v[kWide][kSteps][1];
@@ -79,44 +80,62 @@ __global__ __launch_bounds__(kQuantThreads) void mxfp4_quantize_kernel(const uin
 template <bool BF16, bool STREAM>
 __global__ __launch_bounds__(kQuantThreads) void mxfp4_quantize_columns_kernel(
     const uint8_t* __restrict__ x, int64_t row_bytes, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-    int64_t depth, int64_t width, int64_t slabs, int64_t row_units) {
+    int64_t depth, int64_t width, uint32_t slabs, int64_t row_units, bool across) {
   constexpr int kSize = BF16 ? 2 : 4;
-  const int64_t slab = blockIdx.x % slabs;
-  const int64_t col = blockIdx.x / slabs * 64 + (threadIdx.x & 31) * 2;
+  // neighbours take the slabs of the same columns, or (across) the same rows' next columns
+  const uint32_t groups = (uint32_t)((width + 63) / 64), inner = across ? groups : slabs;
+  const uint32_t outer_at = blockIdx.x / inner, inner_at = blockIdx.x - outer_at * inner;
+  const uint32_t slab = across ? outer_at : inner_at, group = across ? inner_at : outer_at;
+  const int64_t col = (int64_t)group * 64 + (threadIdx.x & 31) * 2;
   const int b = threadIdx.x >> 5;
-  const int64_t k0 = slab * kMxSlab + b * 32;
+  const int64_t k0 = (int64_t)slab * kMxSlab + b * 32;
   const int64_t unit_row = col / kMxRows;
   if (unit_row >= row_units) return;
-  const uint8_t* p = x + k0 * row_bytes + col * kSize;
   float v[2][32];
+  auto load = [&](const uint8_t* p, int k) __attribute__((always_inline)) {
+    if constexpr (BF16) {
+      const u32_any* at = reinterpret_cast<const u32_any*>(p);
+      const uint32_t w = STREAM ? __builtin_nontemporal_load(at) : *at;
+      v[0][k] = bf16_lo(w);
+      v[1][k] = bf16_hi(w);
+    } else {
+      const u32x2_any* at = reinterpret_cast<const u32x2_any*>(p);
+      const u32x2 w = STREAM ? __builtin_nontemporal_load(at) : *at;
+      v[0][k] = __uint_as_float(w.x);
+      v[1][k] = __uint_as_float(w.y);
+    }
+  };
   if (col + 1 < width && k0 + 32 <= depth) {
+    const uint8_t* p = x + k0 * row_bytes + col * kSize;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) load(p + k * row_bytes, k);
+  } else if (width > 1) {
+    // The last row and the last pair of columns again for what lies behind them, cleared afterwards: loads under
+    // branches would wait for one another (1001 x 4000 bf16: 8.0 us, so 5.3).
+    const int64_t first = col < width - 2 ? col : width - 2, past = col - first;
+    int64_t at = (k0 < depth ? k0 : depth - 1) * row_bytes + first * kSize;
+    const int rows = k0 < depth ? (depth - k0 < 32 ? (int)(depth - k0) : 32) : 0;
 #pragma unroll
     for (int k = 0; k < 32; ++k) {
-      if constexpr (BF16) {
-        const u32_any* at = reinterpret_cast<const u32_any*>(p + k * row_bytes);
-        const uint32_t w = STREAM ? __builtin_nontemporal_load(at) : *at;
-        v[0][k] = bf16_lo(w);
-        v[1][k] = bf16_hi(w);
-      } else {
-        const u32x2_any* at = reinterpret_cast<const u32x2_any*>(p + k * row_bytes);
-        const u32x2 w = STREAM ? __builtin_nontemporal_load(at) : *at;
-        v[0][k] = __uint_as_float(w.x);
-        v[1][k] = __uint_as_float(w.y);
-      }
+      load(x + at, k);
+      at += k + 1 < rows ? row_bytes : 0;
+      asm volatile("" : "+v"(at));                 // (one running address, not 32)
+    }
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      const bool there = k < rows;
+      v[0][k] = there && past < 2 ? (past == 1 ? v[1][k] : v[0][k]) : 0.0f;
+      v[1][k] = there && past == 0 ? v[1][k] : 0.0f;
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < 32; ++k)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        v[c][k] = 0.0f;
-        if (col + c < width && k0 + k < depth) {
-          if constexpr (BF16)
-            v[c][k] = __uint_as_float((uint32_t) reinterpret_cast<const uint16_t*>(p + k * row_bytes)[c] << 16);
-          else
-            v[c][k] = reinterpret_cast<const float*>(p + k * row_bytes)[c];
-        }
+    for (int k = 0; k < 32; ++k) {
+      v[0][k] = v[1][k] = 0.0f;
+      if (col == 0 && k0 + k < depth) {
+        if constexpr (BF16) v[0][k] = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(x + (k0 + k) * row_bytes) << 16);
+        else v[0][k] = *reinterpret_cast<const float*>(x + (k0 + k) * row_bytes);
       }
+    }
   }
   const int64_t unit = mx_unit(unit_row, slab, row_units);
 #pragma unroll
@@ -152,13 +171,14 @@ template <bool BF16, bool STREAM>
 __global__ __launch_bounds__(kQuantThreads) void mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes,
                                                                         const uint8_t* __restrict__ scales,
                                                                         uint8_t* __restrict__ out, int64_t rows,
-                                                                        int64_t cols, int64_t slabs, int64_t units) {
+                                                                        int64_t cols, uint32_t slabs, uint32_t units) {
   constexpr int kSize = BF16 ? 2 : 4;
   const int lane = threadIdx.x & 63;
-  const int64_t at = (int64_t)blockIdx.x * (kQuantThreads / 64) + (threadIdx.x >> 6);
+  const uint32_t at = blockIdx.x * (kQuantThreads / 64) + (threadIdx.x >> 6);
   if (at >= units) return;
-  const int64_t row0 = at / slabs * kMxRows, col0 = at % slabs * kMxSlab;
-  const int64_t unit = mx_unit(at / slabs, at % slabs, units / slabs);
+  const uint32_t row_unit = at / slabs, slab = at - row_unit * slabs;
+  const int64_t row0 = (int64_t)row_unit * kMxRows, col0 = (int64_t)slab * kMxSlab;
+  const int64_t unit = mx_unit(row_unit, slab, units / slabs);
   const int col = (lane & 31) * 8, b = (lane & 31) >> 2, q = lane & 3;
   const int64_t left = cols - col0 - col;
   if (left <= 0) return;
@@ -249,15 +269,18 @@ int smr_mxfp4_quantize(const void* x_dev, int64_t row_stride, void* codes_dev, v
   uint8_t* scales = static_cast<uint8_t*>(scales_dev);
   // Past the caches from 64 MiB on: what the caches can hold may be there (4096 x 4096 bf16 9.3 us, streamed
   // 10.0), what they cannot only drives the codes out of them (16384 x 8192 64 us, streamed 55; along
-  // the columns 75 and 65; with the codes read back behind it 164 and 133).
+  // the columns bf16 75 and 65; with the codes read back behind it 164 and 133).
   const bool stream = rows * cols * size >= ((int64_t)64 << 20);
   if (transpose) {
     const int64_t slabs = mx_slabs(rows), row_units = mx_row_units(cols);
     const int64_t grid = (cols + 63) / 64 * slabs;
     if (grid > kMxMaxGrid) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_quantize: too large for one launch");
+    // Large fp32 inputs across the rows (16384 x 8192 106 us, down the columns 122; 8191 x 3584 26.6 and 27.9; 4096 x
+    // 4096 15.6 and 13.9; 16384 x 8192 bf16 69 and 65).
+    const bool across = !bf16 && rows * cols * size > ((int64_t)96 << 20);
 #define SMR_QUANT(B, S)                                                                                                \
   hipLaunchKernelGGL((mxfp4_quantize_columns_kernel<B, S>), dim3((unsigned)grid), dim3(kQuantThreads), 0, s, x,        \
-                     row_stride * size, codes, scales, rows, cols, slabs, row_units)
+                     row_stride * size, codes, scales, rows, cols, (uint32_t)slabs, row_units, across)
     if (bf16 && stream) SMR_QUANT(true, true);
     else if (bf16) SMR_QUANT(true, false);
     else if (stream) SMR_QUANT(false, true);
@@ -269,7 +292,7 @@ int smr_mxfp4_quantize(const void* x_dev, int64_t row_stride, void* codes_dev, v
     if (grid > kMxMaxGrid) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_quantize: too large for one launch");
 #define SMR_QUANT(B, S)                                                                                             \
   hipLaunchKernelGGL((mxfp4_quantize_kernel<B, S>), dim3((unsigned)grid), dim3(kQuantThreads), 0, s, x,             \
-                     row_stride * size, codes, scales, rows, cols, slabs, units)
+                     row_stride * size, codes, scales, rows, cols, (uint32_t)slabs, (uint32_t)units)
     if (bf16 && stream) SMR_QUANT(true, true);
     else if (bf16) SMR_QUANT(true, false);
     else if (stream) SMR_QUANT(false, true);
@@ -308,7 +331,7 @@ int smr_mxfp4_dequantize(const void* codes_dev, const void* scales_dev, void* ou
                       rows * cols * size >= ((int64_t)128 << 20);
 #define SMR_DEQUANT(B, S)                                                                                            \
   hipLaunchKernelGGL((mxfp4_dequantize_kernel<B, S>), dim3((unsigned)grid), dim3(kQuantThreads), 0, s, codes, scales, \
-                     out, rows, cols, slabs, units)
+                     out, rows, cols, (uint32_t)slabs, (uint32_t)units)
   if (bf16 && stream) SMR_DEQUANT(true, true);
   else if (bf16) SMR_DEQUANT(true, false);
   else if (stream) SMR_DEQUANT(false, true);

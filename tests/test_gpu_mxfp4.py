@@ -20,7 +20,7 @@ def _same_operand(q, codes, scales):
     assert torch.equal(got_codes.cpu(), codes)
 
 
-SIZES = [(1, 1), (1, 32), (1, 8192), (2, 33), (15, 255), (16, 256), (17, 257), (3, 1001), (64, 96), (300, 700), (129, 4100)]
+SIZES = [(1, 1), (1, 32), (1, 8192), (2, 33), (15, 255), (16, 256), (17, 257), (3, 1001), (64, 96), (300, 700), (129, 4100), (300, 1), (45, 2), (289, 3)]
 
 
 @pytest.mark.parametrize("rows,cols", SIZES)
