@@ -166,7 +166,7 @@ __device__ __forceinline__ void put_vec(uint8_t* p, const u32x4& v) {
 }
 
 // Back to rows of bf16 or fp32 (both hold every value exactly: two significant bits, exponents
-// from -128 to 127).  The mapping of the quantiser: a wave takes a unit, 8 values per lane.
+// from -128 to 127).  A wave takes a unit, 8 values per lane, two rows at a time.
 template <bool BF16, bool STREAM>
 __global__ __launch_bounds__(kQuantThreads) void mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes,
                                                                         const uint8_t* __restrict__ scales,

@@ -400,7 +400,8 @@ __global__ __launch_bounds__(kSumThreads) void norm_sums_kernel(const float* __r
 
 // Rows that one workgroup takes, one after the other, instead of one workgroup each and a second launch for
 // their sums: 3 x 4096 8.0 us and 7.8, 5 x 4096 11.0 and 7.7 - but the second launch and its scratch array
-// cost a caller on the host another 4.4 us.
+// cost a caller on the host another 4.4 us.  (As many rows at a time as 1024 threads have room for, their sums
+// joined in LDS: 16 x 512 10.4 us against 6.4 in two launches, 40 x 1000 30 against 8.2.)
 constexpr int kOneWorkgroupRows = 5;
 
 // How a backward pass is launched; `parts` > 1 leave cols fp32 sums per kind each.

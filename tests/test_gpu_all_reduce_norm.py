@@ -186,6 +186,11 @@ BACKWARD = [
     ((2, 8200), "bf16", True, "element", 1.0, True), ((2, 16384), "bf16", True, "channel", 1.0, True),
     ((2, 16383), "bf16", True, "token", 1.0, True), ((2, 16381), "fp32", True, "channel", 1.0, True),
     ((1030, 2048), "bf16", True, "token", 1.0, True), ((5000, 40), "fp32", True, "element", 1.0, True),
+    # one workgroup, several rows at a time, the last turn full and not
+    ((80, 512), "bf16", True, "channel", 1.0, True), ((79, 499), "bf16", True, "token", 1.0, False), ((40, 1000), "bf16", False, "channel", 1.0, True),
+    ((33, 777), "bf16", True, "element", 2.0, True), ((20, 2048), "bf16", True, "none", 1.0, True), ((10, 4001), "bf16", True, "channel", 1.0, True),
+    ((65, 250), "fp32", True, "channel", 1.0, True), ((17, 300), "fp32", False, "token", 1.0, True), ((9, 2048), "fp32", True, "element", 1.0, False),
+    ((6, 8), "bf16", True, "channel", 1.0, True), ((13, 1023), "fp32", True, "token", 1.0, True), ((5, 1536), "bf16", True, "element", 1.0, True),
     # several rows per workgroup: rows ahead of one and of two vectors a thread, rows kept, rows read again
     ((600, 4096), "bf16", False, "channel", 1.0, False), ((520, 8192), "bf16", True, "channel", 1.0, True),
     ((530, 8001), "bf16", True, "element", 1.0, True), ((513, 2999), "bf16", True, "none", -1.0, True),
