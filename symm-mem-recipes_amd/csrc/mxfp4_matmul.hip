@@ -833,27 +833,30 @@ static int launch_ring(const MxOperands& o, hipStream_t s) {
 
 // Which kernel: the one with the lowest estimate of its time in microseconds, fitted to launches on 256 compute
 // units.  A launch costs a few microseconds to start and drain; a pass of the chip over one tile per compute unit
-// costs its first loads and stores and so much per slab, a pass that is not full at least 0.6 of that; the two kernels
-// without a persistent grid are bound by latency while they fill the chip once.
+// costs its first loads and stores and so much per slab, a last one that is not full 0.6 of that and up, less the
+// more passes went before it (the workgroups drift apart); the two kernels without a persistent grid are bound by
+// latency while they fill the chip once.
 //                     n slabs           M x 3584: time (us) of few / 64x128 / 128x128 / 256x128 / 256x224
 //   few    64 x 32    0.75 + 0.117 n     512, K = 8192:  20.5 / 17.5 / 19.8 / 24.6 / 37.3    K = 768:  6.6 /  5.1 /  6.2 /  8.4 / 12.3
 //   ring   64 x 128   1.3  + 0.35  n    1024            33.5 / 25.7 / 22.0 / 27.2 / 38.9             10.9 /  7.2 /  6.9 /  9.0 / 12.8
 //   tiles 128 x 128   2.9  + 0.525 n    2048            66   / 50   / 42   / 34.3 / 45.2             19.0 / 12.0 / 12.0 / 10.7 / 14.4
-//   tiles 256 x 128   6    + 0.78  n    4096           130   / 91   / 81   / 65   / 56               34   / 19.6 / 20.4 / 19.6 / 17
+//   tiles 256 x 128   6.5  + 0.82  n    4096           130   / 91   / 81   / 65   / 56               34   / 19.6 / 20.4 / 19.6 / 17
 //   tiles 256 x 224  10.6  + 1.31  n    8192                                                         66   / 35   / 33   / 35   / 31.5
+// 16384 x 8192 x 8192: 256 x 128 531 us, 256 x 224 494.  (A 256 x 256 tile with two slabs of A in LDS in place of
+// three spills a little and gains 2 to 4 % where it fills passes that 224 does not: not kept.)
 enum MxKernel { kMxFew, kMxRing64x128, kMxTile128x128, kMxTile256x128, kMxTile256x224 };
 
 static MxKernel pick_kernel(int64_t M, int64_t N, int64_t slabs, int cus) {
   auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-  auto passes = [&](int64_t bm, int64_t bn) {
-    const int64_t all = tiles(bm, bn), rest = all % cus;
-    return (double)(all / cus) + (rest > 0 ? 0.6 + 0.4 * (double)rest / cus : 0.0);
-  };
   auto larger = [](double a, double b) { return a > b ? a : b; };
+  auto passes = [&](int64_t bm, int64_t bn) {
+    const double full = (double)(tiles(bm, bn) / cus), rest = (double)(tiles(bm, bn) % cus) / cus;
+    return full + (rest > 0 ? larger(rest, 0.6 + 0.4 * rest - 0.06 * full) : 0.0);
+  };
   const double n = (double)slabs;
   const double time[5] = {larger(3.3 + 0.157 * n, 3 + (double)tiles(64, 32) / cus * (0.75 + 0.117 * n)),
                           larger(3.8 + 0.42 * n, 2.5 + passes(64, 128) * (1.3 + 0.35 * n)),
-                          2.4 + passes(128, 128) * (2.9 + 0.525 * n), 3 + passes(256, 128) * (6 + 0.78 * n),
+                          2.4 + passes(128, 128) * (2.9 + 0.525 * n), 1.5 + passes(256, 128) * (6.5 + 0.82 * n),
                           3.5 + passes(256, 224) * (10.6 + 1.31 * n)};
   int best = 0;
   for (int k = 1; k < 5; ++k)
