@@ -243,16 +243,16 @@ __global__ __launch_bounds__(WAVES * 64) void mxfp4_matmul_rows_kernel(
 // 256-thread workgroups, one per compute unit, each computing BM x BN tiles with 4 waves in a
 // 2 x 2 arrangement.  A slab (rows x 256 of K, 128 bytes a row) comes from memory straight into
 // LDS with 128-bit direct-to-LDS loads; operands being in MFMA order, loads and fragment reads
-// are both linear.  LDS holds three slabs of A, two of B and two sets of scales: while one pair
-// of slabs is multiplied, the next is complete or landing and the A slab after that is on its
-// way.  With the bf16 MFMA replaced by one that does four times the work on the same bytes in
+// are both linear.  LDS holds three slabs of A (of a 256 x 256 tile two), two of B and two sets of
+// scales: while one pair of slabs is multiplied, the next is complete or landing and the A slab
+// after that is on its way.  With the bf16 MFMA replaced by one that does four times the work on the same bytes in
 // the same time, the bytes per cycle are those of the bf16 GEMM of ag_matmul.hip, and so is the
 // order of work inside a slab pair (two steps of 128 of K):
 //   first step    MFMAs of step 0; the fragments of step 1 are read; A slab kt+2 is requested
 //   barrier       pair kt is read by everyone, pair kt+1 has landed
 //   second step   MFMAs of step 1; fragments of step 0 and the scales of pair kt+1 are read;
-//                 B slab and scales of pair kt+2 are requested
-// 16384 x 3584 x 8192: 201 us, 4.8 PFLOP/s.  Nothing but its MFMAs on such data takes 149 us (6.5 PFLOP/s: the
+//                 B slab and scales of pair kt+2 (and its A slab where LDS holds two) are requested
+// 16384 x 3584 x 8192: 198 us, 4.9 PFLOP/s.  Nothing but its MFMAs on such data takes 149 us (6.5 PFLOP/s: the
 // clock is power-limited; zeros reach 8.9).  With 32 bytes a row per store it took 224: 187 without the stores, 190
 // without the loads from memory, 178 without those and the fragment reads.  Stores that stay in flight under the next
 // tile's first slabs, and 128 bytes a row per store, were no faster than 64.
@@ -384,8 +384,24 @@ __device__ __forceinline__ int mx_tile_number(int total, int grid, int wg, int p
   return (wg >> 3) < per_xcd && at < count ? (int)start + at : -1;
 }
 
+// A fragment's value where it is used.  IN_ACC: it lies in accumulation registers; left to itself the compiler
+// copies all of a tile to vector registers ahead of the stores (16384 x 8192 x 8192 495 us, so 483; 4096 x 4096 x
+// 4096 52.5 and 50), and a 256 x 256 tile to scratch memory.
+template <bool IN_ACC>
+__device__ __forceinline__ f32x4 fetched(const f32x4& acc) {
+  if constexpr (!IN_ACC) return acc;
+  f32x4 d;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float f;
+    asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(f) : "a"(acc[e]));
+    d[e] = f;
+  }
+  return d;
+}
+
 // A wave's FM x FN fragments to rows m0.., columns n0.. of C.
-template <bool BF16, int FM, int FN>
+template <bool BF16, int FM, int FN, bool IN_ACC>
 __device__ __forceinline__ void store_tile(const MxTiles& p, int64_t m0, int64_t n0, int lane, const f32x4 (&acc)[FN][FM]) {
   constexpr int kSize = BF16 ? 2 : 4;
   const int64_t m_lane = m0 + (lane & 15), n_lane = n0 + (lane >> 4) * 4;
@@ -398,11 +414,11 @@ __device__ __forceinline__ void store_tile(const MxTiles& p, int64_t m0, int64_t
       if (m_lane + mi * 16 < p.M) {
         if constexpr (BF16) {
 #pragma unroll
-          for (int ni = 0; ni + 1 < FN; ni += 2) put8_of_two(out + shift + ni * 16 * kSize, acc[ni][mi], acc[ni + 1][mi]);
-          if constexpr (FN & 1) put4<BF16>(out + (FN - 1) * 16 * kSize, acc[FN - 1][mi]);
+          for (int ni = 0; ni + 1 < FN; ni += 2) put8_of_two(out + shift + ni * 16 * kSize, fetched<IN_ACC>(acc[ni][mi]), fetched<IN_ACC>(acc[ni + 1][mi]));
+          if constexpr (FN & 1) put4<BF16>(out + (FN - 1) * 16 * kSize, fetched<IN_ACC>(acc[FN - 1][mi]));
         } else {
 #pragma unroll
-          for (int ni = 0; ni < FN; ++ni) put4<BF16>(out + ni * 16 * kSize, acc[ni][mi]);
+          for (int ni = 0; ni < FN; ++ni) put4<BF16>(out + ni * 16 * kSize, fetched<IN_ACC>(acc[ni][mi]));
         }
       }
       out += p.N * (16 * kSize);
@@ -414,7 +430,7 @@ __device__ __forceinline__ void store_tile(const MxTiles& p, int64_t m0, int64_t
 #pragma unroll
       for (int ni = 0; ni < FN; ++ni)
         if (m_lane + mi * 16 < p.M && n_lane + ni * 16 < p.N)
-          store4<BF16>(p.c, m_lane + mi * 16, n_lane + ni * 16, p.N, acc[ni][mi]);
+          store4<BF16>(p.c, m_lane + mi * 16, n_lane + ni * 16, p.N, fetched<IN_ACC>(acc[ni][mi]));
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -427,7 +443,9 @@ __global__ __launch_bounds__(kTileThreads, 1) void mxfp4_matmul_tile_kernel(MxTi
   constexpr int kA = BM * 128, kB = BN * 128;           // bytes of a slab
   constexpr int SA = (BM / 16 + 7) / 8, SB = (BN / 16 + 7) / 8;        // 1 KiB loads of scales (8 units each)
   constexpr int kS = (SA + SB) * 1024;
-  constexpr int kOffB = 3 * kA, kOffS = kOffB + 2 * kB;
+  // a third slab of A where LDS has room for it
+  constexpr bool kDeep = 3 * kA + 2 * kB + 2 * kS <= 160 * 1024;
+  constexpr int kOffB = (kDeep ? 3 : 2) * kA, kOffS = kOffB + 2 * kB;
   static_assert(SA + SB <= 4, "one load of scales per wave");
   static_assert(kOffS + 2 * kS <= 160 * 1024, "LDS");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kOffS + 2 * kS];
@@ -525,12 +543,12 @@ __global__ __launch_bounds__(kTileThreads, 1) void mxfp4_matmul_tile_kernel(MxTi
     const uint8_t* bp = b_base + (2 < nk ? 2 : nk - 1) * b_step;
     const uint8_t* sp = s_base + (2 < nk ? 2 : nk - 1) * s_step;
     uint32_t a_at = 0;                           // offset of A slab kt in its ring of three
-    uint32_t a_to = lds0 + 2 * kA + wave * (GA * 1024);      // where A slab kt + 2 goes
+    uint32_t a_to = lds0 + (kDeep ? 2 * kA : 0) + wave * (GA * 1024);        // where A slab kt + 2 goes
 
     constexpr int kMfma = FM * FN, kFrags = FM + FN;
-    using Plan0 = StepPlan<GA, kMfma / GA, kFrags, kMfma * 13 / 16>;
-    constexpr int kGap1 = (kMfma / 2) / GB;
-    using Plan1 = StepPlan<GB + 1, kGap1, 2 * kFrags, kMfma * 15 / 16>;
+    using Plan0 = StepPlan<kDeep ? GA : 0, kMfma / GA, kFrags, kMfma * 13 / 16>;
+    constexpr int kLoads1 = GB + 1 + (kDeep ? 0 : GA), kGap1 = kDeep ? (kMfma / 2) / GB : (kMfma * 3 / 4) / kLoads1;
+    using Plan1 = StepPlan<kLoads1, kGap1, 2 * kFrags, kMfma * 15 / 16>;
     // (the last load of the first step stands at (GA - 1) * (kMfma / GA))
     constexpr bool kRoom = kMfma - 6 >= kMfma * 13 / 16 && kMfma - 6 > (GA - 1) * (kMfma / GA);
     constexpr int kBook = kRoom ? kMfma - 6 : kMfma - 1, kBookGap = kRoom ? 1 : 0;
@@ -550,23 +568,25 @@ __global__ __launch_bounds__(kTileThreads, 1) void mxfp4_matmul_tile_kernel(MxTi
           else bf1[r - FM] = lds_frag(b_fr + 1024 + (r - FM) * 2048);
         });
         // the uniform bookkeeping goes between the last MFMAs, behind the step's loads and reads
-        if constexpr (at == kBook) {
+        if constexpr (at == kBook && kDeep) {
           const uint32_t next = a_at == 2 * kA ? 0 : a_at + kA;
           a_fr += next - a_at;
           a_at = next;
         }
-        if constexpr (at == kBook + kBookGap) a_to = lds0 + wave * (GA * 1024) + (a_at >= kA ? a_at - kA : 2 * kA);
+        if constexpr (at == kBook && !kDeep) a_fr += P == 0 ? (uint32_t)kA : (uint32_t)-kA;
+        if constexpr (at == kBook + kBookGap && kDeep) a_to = lds0 + wave * (GA * 1024) + (a_at >= kA ? a_at - kA : 2 * kA);
         if constexpr (at == kBook + 2 * kBookGap) b_fr += P == 0 ? (uint32_t)kB : (uint32_t)-kB;
         if constexpr (at == kBook + 3 * kBookGap) {
           sa_fr += P == 0 ? (uint32_t)kS : (uint32_t)-kS;
           sb_fr += P == 0 ? (uint32_t)kS : (uint32_t)-kS;
         }
-        if constexpr (at == kBook + 4 * kBookGap) ap += kt + 3 < nk ? a_step : 0;
+        if constexpr (at == kBook + 4 * kBookGap && kDeep) ap += kt + 3 < nk ? a_step : 0;
         __builtin_amdgcn_sched_barrier(0);
       });
-      // this wave's loads of pair kt+1 are complete; those of A slab kt+2 may be in flight
+      // this wave's loads of pair kt+1 are complete; those of A slab kt+2, if any yet, may be in flight
       static_assert(GA == 8 || GA == 4 || GA == 2, "explicit vmcnt below");
-      if constexpr (GA == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      if constexpr (!kDeep) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      else if constexpr (GA == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
       else if constexpr (GA == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
       else asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
       __syncthreads();
@@ -575,6 +595,9 @@ __global__ __launch_bounds__(kTileThreads, 1) void mxfp4_matmul_tile_kernel(MxTi
         if constexpr (Plan1::is_load(at) && g < GB)
           mfma_mx_load<1, g * 1024>(acc[ni][mi], bf1[ni], af1[mi], sb[P][ni], sa[P][mi], bp, b_off[g < GB ? g : 0],
                                     lds0 + kOffB + P * kB + wave * (GB * 1024));
+        else if constexpr (Plan1::is_load(at) && g < kLoads1 - 1)
+          mfma_mx_load<1, P * kA + (g - GB) * 1024>(acc[ni][mi], bf1[ni], af1[mi], sb[P][ni], sa[P][mi], ap,
+                                                    a_off[g - GB < GA && g >= GB ? g - GB : 0], a_to);
         else if constexpr (Plan1::is_load(at))
           mfma_mx_load<1, P * kS>(acc[ni][mi], bf1[ni], af1[mi], sb[P][ni], sa[P][mi], sp, s_off, s_dst);
         else
@@ -593,6 +616,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void mxfp4_matmul_tile_kernel(MxTi
             else sb[1 - P][f - FM] = lds_u16(sb_fr + (f - FM) * 128);
           }
         });
+        if constexpr (at == kMfma - 4 && !kDeep) ap += kt + 3 < nk ? a_step : 0;
         if constexpr (at == kMfma - 3) bp += kt + 3 < nk ? b_step : 0;
         if constexpr (at == kMfma - 2) sp += kt + 3 < nk ? s_step : 0;
         __builtin_amdgcn_sched_barrier(0);
@@ -618,7 +642,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void mxfp4_matmul_tile_kernel(MxTi
     }
     int le = lane;
     asm volatile("" : "+v"(le));
-    store_tile<BF16, FM, FN>(p, m0, n0, le, acc);
+    store_tile<BF16, FM, FN, true>(p, m0, n0, le, acc);
     if (number < 0) return;
   }
 }
@@ -748,7 +772,7 @@ __global__ __launch_bounds__(kTileThreads) void mxfp4_matmul_ring_kernel(MxTiles
   if (kt < nk) turn(even, odd);
   // (LDS is given back when the workgroup ends: nothing may still be landing in it)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  store_tile<BF16, FM, FN>(p, (int64_t)tile_m * BM + wm * (BM / 2), (int64_t)tile_n * BN + wn * (BN / 2), lane, acc);
+  store_tile<BF16, FM, FN, false>(p, (int64_t)tile_m * BM + wm * (BM / 2), (int64_t)tile_n * BN + wn * (BN / 2), lane, acc);
 }
 
 struct MxOperands {
@@ -836,15 +860,14 @@ static int launch_ring(const MxOperands& o, hipStream_t s) {
 // costs its first loads and stores and so much per slab, a last one that is not full 0.6 of that and up, less the
 // more passes went before it (the workgroups drift apart); the two kernels without a persistent grid are bound by
 // latency while they fill the chip once.
-//                     n slabs           M x 3584: time (us) of few / 64x128 / 128x128 / 256x128 / 256x224
-//   few    64 x 32    0.75 + 0.117 n     512, K = 8192:  20.5 / 17.5 / 19.8 / 24.6 / 37.3    K = 768:  6.6 /  5.1 /  6.2 /  8.4 / 12.3
-//   ring   64 x 128   1.3  + 0.35  n    1024            33.5 / 25.7 / 22.0 / 27.2 / 38.9             10.9 /  7.2 /  6.9 /  9.0 / 12.8
-//   tiles 128 x 128   2.9  + 0.525 n    2048            66   / 50   / 42   / 34.3 / 45.2             19.0 / 12.0 / 12.0 / 10.7 / 14.4
-//   tiles 256 x 128   6.5  + 0.82  n    4096           130   / 91   / 81   / 65   / 56               34   / 19.6 / 20.4 / 19.6 / 17
-//   tiles 256 x 224  10.6  + 1.31  n    8192                                                         66   / 35   / 33   / 35   / 31.5
-// 16384 x 8192 x 8192: 256 x 128 531 us, 256 x 224 494.  (A 256 x 256 tile with two slabs of A in LDS in place of
-// three spills a little and gains 2 to 4 % where it fills passes that 224 does not: not kept.)
-enum MxKernel { kMxFew, kMxRing64x128, kMxTile128x128, kMxTile256x128, kMxTile256x224 };
+//                     n slabs           M x 3584: us of few / 64x128 / 128x128 / 256x128 / 256x224 / 256x256
+//   few    64 x 32    0.75 + 0.117 n     512, K = 8192:  20.5 / 17.9 / 20.0 / 25 / 37 / 45    K = 768:  6.6 /  5.1 /  6.0 /  7.9 / 11.3 / 12.0
+//   ring   64 x 128   1.3  + 0.35  n    1024            33.5 / 25.9 / 21.8 / 26 / 38 / 46             10.9 /  7.2 /  6.7 /  8.7 / 12.0 / 12.6
+//   tiles 128 x 128   2.7  + 0.53  n    2048            66   / 50   / 41   / 33 / 42 / 48             19.0 / 12.2 / 11.7 / 10.4 / 13.7 / 14.2
+//   tiles 256 x 128   5.2  + 0.87  n    4096           130   / 91   / 80   / 63 / 54 / 57             34   / 19.7 / 19.5 / 16.8 / 15.2 / 15.7
+//   tiles 256 x 224   8.8  + 1.34  n    8192                                                          66   / 35   / 31   / 29.7 / 28.0 / 27.0
+//   tiles 256 x 256   9.7  + 1.54  n    (4096 x 4096 x 4096: 58 / 48 / 42 / 50 / 36.6 from 64x128 on; 8192 x 8192 x 8192: 405 / 350 / 278 / 250 / 242)
+enum MxKernel { kMxFew, kMxRing64x128, kMxTile128x128, kMxTile256x128, kMxTile256x224, kMxTile256x256 };
 
 static MxKernel pick_kernel(int64_t M, int64_t N, int64_t slabs, int cus) {
   auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
@@ -854,12 +877,12 @@ static MxKernel pick_kernel(int64_t M, int64_t N, int64_t slabs, int cus) {
     return full + (rest > 0 ? larger(rest, 0.6 + 0.4 * rest - 0.06 * full) : 0.0);
   };
   const double n = (double)slabs;
-  const double time[5] = {larger(3.3 + 0.157 * n, 3 + (double)tiles(64, 32) / cus * (0.75 + 0.117 * n)),
+  const double time[6] = {larger(3.3 + 0.157 * n, 3 + (double)tiles(64, 32) / cus * (0.75 + 0.117 * n)),
                           larger(3.8 + 0.42 * n, 2.5 + passes(64, 128) * (1.3 + 0.35 * n)),
-                          2.4 + passes(128, 128) * (2.9 + 0.525 * n), 1.5 + passes(256, 128) * (6.5 + 0.82 * n),
-                          3.5 + passes(256, 224) * (10.6 + 1.31 * n)};
+                          2.4 + passes(128, 128) * (2.7 + 0.53 * n), 2.5 + passes(256, 128) * (5.2 + 0.87 * n),
+                          2.3 + passes(256, 224) * (8.8 + 1.34 * n), 2.5 + passes(256, 256) * (9.7 + 1.54 * n)};
   int best = 0;
-  for (int k = 1; k < 5; ++k)
+  for (int k = 1; k < 6; ++k)
     if (time[k] < time[best]) best = k;
   return (MxKernel)best;
 }
@@ -887,7 +910,8 @@ static int launch_matmul(const MxOperands& o, hipStream_t s) {
     case kMxRing64x128: return launch_ring<BF16, 64, 128, 3>(o, s);
     case kMxTile128x128: return launch_tiles<BF16, 128, 128>(o, s);
     case kMxTile256x128: return launch_tiles<BF16, 256, 128>(o, s);
-    default: return launch_tiles<BF16, 256, 224>(o, s);
+    case kMxTile256x224: return launch_tiles<BF16, 256, 224>(o, s);
+    default: return launch_tiles<BF16, 256, 256>(o, s);
   }
 }
 
