@@ -252,7 +252,7 @@ __global__ __launch_bounds__(WAVES * 64) void mxfp4_matmul_rows_kernel(
 //   barrier       pair kt is read by everyone, pair kt+1 has landed
 //   second step   MFMAs of step 1; fragments of step 0 and the scales of pair kt+1 are read;
 //                 B slab and scales of pair kt+2 (and its A slab where LDS holds two) are requested
-// 16384 x 3584 x 8192: 198 us, 4.9 PFLOP/s.  Nothing but its MFMAs on such data takes 149 us (6.5 PFLOP/s: the
+// 16384 x 3584 x 8192: 201 us, 4.8 PFLOP/s.  Nothing but its MFMAs on such data takes 149 us (6.5 PFLOP/s: the
 // clock is power-limited; zeros reach 8.9).  With 32 bytes a row per store it took 224: 187 without the stores, 190
 // without the loads from memory, 178 without those and the fragment reads.  Stores that stay in flight under the next
 // tile's first slabs, and 128 bytes a row per store, were no faster than 64.
