@@ -415,7 +415,8 @@ int64_t smr_norm_backward_scratch_bytes(int64_t rows, int64_t cols, int dtype, i
  *           l & 15, elements 32 * (l >> 4) .. + 31 of the step's 128, the first of a pair in the
  *           low half of its byte
  *   scales  [ceil(cols/256)][ceil(rows/16)][64 lanes][2 steps] biased exponents, 255 = NaN
- * with zeros where a unit reaches past rows or cols. */
+ * with zeros where a unit reaches past rows or cols.  Both are aligned to 16 bytes; what a call of
+ * the functions below writes lies apart from what it reads. */
 int64_t smr_mxfp4_code_bytes(int64_t rows, int64_t cols);
 int64_t smr_mxfp4_scale_bytes(int64_t rows, int64_t cols);
 
