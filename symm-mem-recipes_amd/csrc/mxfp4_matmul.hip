@@ -263,7 +263,9 @@ constexpr int kTileThreads = 256;
 __device__ __forceinline__ i32x4 lds_frag(uint32_t addr) {
   return *reinterpret_cast<__attribute__((address_space(3))) const i32x4*>((uintptr_t)addr);
 }
-__device__ __forceinline__ uint16_t lds_u16(uint32_t addr) {
+// (32 bits wide from the load on: the compiler would widen a 16-bit value in front of the MFMA that takes it, and an
+// MFMA in assembly has to be two wait states behind a vector instruction that writes one of its operands)
+__device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
   return *reinterpret_cast<__attribute__((address_space(3))) const uint16_t*>((uintptr_t)addr);
 }
 // A pointer that is the same in every lane, kept in scalar registers.
@@ -286,8 +288,8 @@ __device__ __forceinline__ void load_kib(const uint8_t* base, uint32_t voff, uin
 // move the accumulators between the register files inside the loop.  STEP picks the byte of the
 // scale registers.
 template <int STEP>
-__device__ __forceinline__ void mfma_mx_acc(f32x4& acc, const i32x4& first, const i32x4& second, uint16_t first_scale,
-                                            uint16_t second_scale) {
+__device__ __forceinline__ void mfma_mx_acc(f32x4& acc, const i32x4& first, const i32x4& second, uint32_t first_scale,
+                                            uint32_t second_scale) {
   if constexpr (STEP == 0)
     asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
                  : "+a"(acc)
@@ -302,8 +304,8 @@ __device__ __forceinline__ void mfma_mx_acc(f32x4& acc, const i32x4& first, cons
 // an issue slot, and an MFMA lasts four of them: the write of M0 stands ahead of the MFMA, which is
 // the distance the load needs from it.
 template <int STEP, int OFFSET>
-__device__ __forceinline__ void mfma_mx_load(f32x4& acc, const i32x4& first, const i32x4& second, uint16_t first_scale,
-                                             uint16_t second_scale, const uint8_t* base, uint32_t voff,
+__device__ __forceinline__ void mfma_mx_load(f32x4& acc, const i32x4& first, const i32x4& second, uint32_t first_scale,
+                                             uint32_t second_scale, const uint8_t* base, uint32_t voff,
                                              uint32_t lds_dst) {
   if constexpr (STEP == 0)
     asm volatile(
@@ -527,7 +529,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void mxfp4_matmul_tile_kernel(MxTi
     uint32_t sa_fr = lds0 + kOffS + (uint32_t)(wm * FM * 128 + ln * 2);
     uint32_t sb_fr = lds0 + kOffS + SA * 1024 + (uint32_t)(wn * FN * 128 + ln * 2);
     i32x4 af0[FM], bf0[FN], af1[FM], bf1[FN];
-    uint16_t sa[2][FM], sb[2][FN];               // by parity of the slab pair
+    uint32_t sa[2][FM], sb[2][FN];               // by parity of the slab pair
 #pragma unroll
     for (int f = 0; f < FM; ++f) af0[f] = lds_frag(a_fr + f * 2048);
 #pragma unroll
