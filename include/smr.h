@@ -440,7 +440,7 @@ int smr_mxfp4_matmul(const void* a_codes_dev, const void* a_scales_dev, const vo
 /* smr_mxfp4_matmul for a few rows of A still in bf16 or fp32 (x [M, K], row_stride elements from row
  * to row), quantised on the way to the codes and scales that smr_mxfp4_quantize writes; the fp32 sum
  * may run in another order than smr_mxfp4_matmul's.  M up to smr_mxfp4_matmul_rows_limit(K): 16, fewer beyond K = 5632, none beyond
- * 90112 (they are kept in LDS). */
+ * 90112 (they are kept in LDS); N up to 2^28 - 64. */
 int64_t smr_mxfp4_matmul_rows_limit(int64_t K);
 int smr_mxfp4_matmul_rows(const void* x_dev, int64_t row_stride, int dtype, const void* b_codes_dev,
                           const void* b_scales_dev, void* c_dev, int64_t M, int64_t N, int64_t K, int out_dtype,

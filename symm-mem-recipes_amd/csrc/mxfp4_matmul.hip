@@ -783,11 +783,14 @@ struct MxOperands {
   int64_t M, N, K;
 };
 
+// The few-rows kernel's grid: groups of rows in y, groups of columns in x.
+static bool few_fits(int64_t m_groups, int64_t n_groups) { return m_groups <= 65535 && n_groups <= kMxMaxGrid / 4; }
+
 template <bool BF16, int TG, int NG, int WAVES>
 static int launch_few(const MxOperands& o, hipStream_t s) {
   const int64_t m_units = mx_row_units(o.M), n_units = mx_row_units(o.N);
   const int64_t gx = (n_units + NG - 1) / NG, gy = (m_units + TG - 1) / TG;
-  if (gx > kMxMaxGrid / 4 || gy > 65535) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul: too large for one launch");
+  if (!few_fits(gy, gx)) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul: too large for one launch");
   hipLaunchKernelGGL((mxfp4_matmul_few_kernel<BF16, TG, NG, WAVES>), dim3((unsigned)gx, (unsigned)gy),
                      dim3(WAVES * 64), 0, s, o.a_codes, o.a_scales, o.b_codes, o.b_scales, o.c, o.M, o.N,
                      mx_slabs(o.K), m_units, n_units);
@@ -803,11 +806,12 @@ struct MxRows {
 };
 // Rows times slabs whose codes and scales (136 B each) fit a workgroup's LDS beside the partial sums.
 constexpr int kRowsLdsUnits = 352;
+// Columns that one launch of four units of columns per workgroup takes.
+constexpr int64_t kRowsMaxN = kMxMaxGrid / 4 * 4 * kMxRows;
 
 template <bool BF16, bool XBF16, int NG, int WAVES>
 static int launch_rows_as(const MxRows& o, hipStream_t s) {
   const int64_t n_units = mx_row_units(o.N), slabs = mx_slabs(o.K), grid = (n_units + NG - 1) / NG;
-  if (grid > kMxMaxGrid / 4) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul_rows: too large for one launch");
   hipLaunchKernelGGL((mxfp4_matmul_rows_kernel<BF16, XBF16, NG, WAVES>), dim3((unsigned)grid), dim3(WAVES * 64),
                      (size_t)(slabs * o.M * 136), s, o.x, o.row_bytes, o.b_codes, o.b_scales, o.c, (int)o.M, o.N, o.K,
                      (int)slabs, n_units);
@@ -837,11 +841,12 @@ static MxTiles tiles_of(const MxOperands& o) {
 }
 
 // Grids are multiples of 8, so that a workgroup's number says which XCD it is on.
+constexpr int64_t kMxMaxTiles = kMxMaxGrid - 8;
 template <bool BF16, int BM, int BN>
 static int launch_tiles(const MxOperands& o, hipStream_t s) {
   const MxTiles t = tiles_of<BM, BN>(o);
   const int64_t total = (int64_t)t.tiles_m * t.tiles_n, cus = compute_units() / 8 * 8;
-  if (total > kMxMaxGrid) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul: too large for one launch");
+  if (total > kMxMaxTiles) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul: too large for one launch");
   const int64_t grid = total < cus ? (total + 7) / 8 * 8 : cus;
   hipLaunchKernelGGL((mxfp4_matmul_tile_kernel<BF16, BM, BN>), dim3((unsigned)grid), dim3(kTileThreads), 0, s, t);
   return check_hip(hipGetLastError(), "smr_mxfp4_matmul launch");
@@ -851,7 +856,7 @@ template <bool BF16, int BM, int BN, int BUFFERS>
 static int launch_ring(const MxOperands& o, hipStream_t s) {
   const MxTiles t = tiles_of<BM, BN>(o);
   const int64_t total = (int64_t)t.tiles_m * t.tiles_n;
-  if (total > kMxMaxGrid - 8) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul: too large for one launch");
+  if (total > kMxMaxTiles) return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul: too large for one launch");
   hipLaunchKernelGGL((mxfp4_matmul_ring_kernel<BF16, BM, BN, BUFFERS>), dim3((unsigned)((total + 7) / 8 * 8)),
                      dim3(kTileThreads), 0, s, t);
   return check_hip(hipGetLastError(), "smr_mxfp4_matmul launch");
@@ -869,10 +874,14 @@ static int launch_ring(const MxOperands& o, hipStream_t s) {
 //   tiles 256 x 128   5.2  + 0.87  n    4096           130   / 91   / 80   / 63 / 54 / 57             34   / 19.7 / 19.5 / 16.8 / 15.2 / 15.7
 //   tiles 256 x 224   8.8  + 1.34  n    8192                                                          66   / 35   / 31   / 29.7 / 28.0 / 27.0
 //   tiles 256 x 256   9.7  + 1.54  n    (4096 x 4096 x 4096: 58 / 48 / 42 / 50 / 36.6 from 64x128 on; 8192 x 8192 x 8192: 405 / 350 / 278 / 250 / 242)
+// A kernel whose grid cannot be launched is no candidate: narrow results are best off with the first at any height, but
+// its groups of rows end at 65535.
 enum MxKernel { kMxFew, kMxRing64x128, kMxTile128x128, kMxTile256x128, kMxTile256x224, kMxTile256x256 };
 
 static MxKernel pick_kernel(int64_t M, int64_t N, int64_t slabs, int cus) {
   auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+  const bool fits[6] = {few_fits((M + 63) / 64, (N + 31) / 32), tiles(64, 128) <= kMxMaxTiles, tiles(128, 128) <= kMxMaxTiles,
+                        tiles(256, 128) <= kMxMaxTiles, tiles(256, 224) <= kMxMaxTiles, tiles(256, 256) <= kMxMaxTiles};
   auto larger = [](double a, double b) { return a > b ? a : b; };
   auto passes = [&](int64_t bm, int64_t bn) {
     const double full = (double)(tiles(bm, bn) / cus), rest = (double)(tiles(bm, bn) % cus) / cus;
@@ -883,9 +892,9 @@ static MxKernel pick_kernel(int64_t M, int64_t N, int64_t slabs, int cus) {
                           larger(3.8 + 0.42 * n, 2.5 + passes(64, 128) * (1.3 + 0.35 * n)),
                           2.4 + passes(128, 128) * (2.7 + 0.53 * n), 2.5 + passes(256, 128) * (5.2 + 0.87 * n),
                           2.3 + passes(256, 224) * (8.8 + 1.34 * n), 2.5 + passes(256, 256) * (9.7 + 1.54 * n)};
-  int best = 0;
-  for (int k = 1; k < 6; ++k)
-    if (time[k] < time[best]) best = k;
+  int best = kMxTile256x256;                         // the fewest workgroups
+  for (int k = kMxTile256x224; k >= kMxFew; --k)
+    if (fits[k] && time[k] <= time[best]) best = k;
   return (MxKernel)best;
 }
 
@@ -902,7 +911,7 @@ static int launch_matmul(const MxOperands& o, hipStream_t s) {
   const int64_t slabs = mx_slabs(o.K);
   const bool wide = o.N > 16384;
   if (o.M <= 16 && !wide) return launch_few<BF16, 1, 1, 8>(o, s);
-  if (o.M <= 16 && slabs < 8) return launch_few<BF16, 1, 4, 8>(o, s);
+  if (o.M <= 16 && slabs < 8 && o.N <= kRowsMaxN) return launch_few<BF16, 1, 4, 8>(o, s);
   if (o.M <= 64 && wide) return launch_ring<BF16, 64, 128, 3>(o, s);
   if (o.M <= 32) return o.N <= 4096 ? launch_few<BF16, 2, 1, 8>(o, s) : launch_few<BF16, 2, 2, 8>(o, s);
   if (o.M <= 48) return o.N <= 4096 ? launch_few<BF16, 3, 1, 8>(o, s) : launch_few<BF16, 3, 2, 8>(o, s);
@@ -960,6 +969,8 @@ int smr_mxfp4_matmul_rows(const void* x_dev, int64_t row_stride, int dtype, cons
     return fail(SMR_E_INVALID, "smr_mxfp4_matmul_rows: N must be in 0..2^31-1, K in 1..2^31-1");
   if (M > smr_mxfp4_matmul_rows_limit(K))
     return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul_rows: more rows than smr_mxfp4_matmul_rows_limit (quantise them first)");
+  if (N > kRowsMaxN)
+    return fail(SMR_E_UNSUPPORTED, "smr_mxfp4_matmul_rows: more than 2^28 - 64 columns (quantise the rows first)");
   if (M > 1 && row_stride < K) return fail(SMR_E_INVALID, "smr_mxfp4_matmul_rows: rows must not overlap (row_stride < K)");
   if (M == 0 || N == 0) return 0;
   if (x_dev == nullptr || b_codes_dev == nullptr || b_scales_dev == nullptr || c_dev == nullptr)

@@ -23,6 +23,8 @@ from . import _lib
 
 #: elements that share a scale; rows and contracted extent of a storage unit
 BLOCK, UNIT_ROWS, SLAB = 32, 16, 256
+#: rows of ``b`` that the product of a few bf16 or fp32 rows takes in one launch
+_ROWS_MAX_N = 2 ** 28 - 64
 
 _DTYPE_CODE = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_FP32}
 #: the current stream's handle without building a torch.cuda.Stream object around it
@@ -226,7 +228,7 @@ def mxfp4_matmul(a: Union[MxFp4Tensor, torch.Tensor], b: MxFp4Tensor, *, out_dty
         out_dtype = out.dtype
     lib = _lib.load()
     if not quantised:
-        if M <= UNIT_ROWS and M <= lib.smr_mxfp4_matmul_rows_limit(b.cols):
+        if M <= UNIT_ROWS and N <= _ROWS_MAX_N and M <= lib.smr_mxfp4_matmul_rows_limit(b.cols):
             row_stride = _check_rows(a)
             _call(a.get_device(), "mxfp4_matmul", lib.smr_mxfp4_matmul_rows, a.data_ptr(), row_stride, _DTYPE_CODE[a.dtype],
                   *b._ptrs(), out.data_ptr(), M, N, b.cols, _DTYPE_CODE[out_dtype])

@@ -184,3 +184,10 @@ def test_the_oracle_of_the_gradients(gate_shape, post):
             want = next(grads)
             want = want[0] if name == "partial" else want
             assert torch.allclose(got[name].reshape(want.shape), want, rtol=1e-10, atol=1e-12), name
+
+
+def test_the_columns_of_the_few_rows_product_end_below_2_to_28(lib):
+    p, f = 0x1000, lib.smr_mxfp4_matmul_rows
+    assert f(p, 32, 0, p, p, p, 1, 2 ** 28 - 63, 32, 0, None) == -2
+    assert b"columns" in lib.smr_last_error_string()
+    assert f(p, 32, 0, p, p, p, 0, 2 ** 28 - 64, 32, 0, None) == 0               # no rows: no launch
