@@ -64,6 +64,11 @@ def _units(rows: int, cols: int) -> int:
     return -(-rows // UNIT_ROWS) * -(-cols // SLAB)
 
 
+def _check_extents(rows: int, cols: int) -> None:
+    assert 0 <= rows < 2 ** 31 and 0 <= cols < 2 ** 31, "rows and cols must be in 0..2^31-1"
+    assert rows or cols, "rows and cols must not both be 0"
+
+
 class MxFp4Tensor:
     """A matrix ``[rows, cols]`` in 4-bit microscaled floats, ``cols`` the axis that a product
     contracts, kept in the order the matrix cores take it (``smr.h``: ``smr_mxfp4_code_bytes``).
@@ -74,7 +79,7 @@ class MxFp4Tensor:
 
     def __init__(self, storage: torch.Tensor, rows: int, cols: int):
         """``storage`` as smr.h lays it out, 16-byte aligned."""
-        assert 0 <= rows < 2 ** 31 and 1 <= cols < 2 ** 31, "rows must be in 0..2^31-1, cols in 1..2^31-1"
+        _check_extents(rows, cols)
         assert storage.dtype == torch.uint8 and storage.is_contiguous(), "storage must be contiguous uint8"
         assert storage.shape == (_units(rows, cols) * 2176,), "storage must be [units * 2176]"
         assert storage.data_ptr() % 16 == 0, "storage must be aligned to 16 bytes"
@@ -106,7 +111,7 @@ class MxFp4Tensor:
     @staticmethod
     def empty(rows: int, cols: int, device) -> "MxFp4Tensor":
         """Storage for a matrix, its values undefined."""
-        assert 0 <= rows < 2 ** 31 and 1 <= cols < 2 ** 31, "rows must be in 0..2^31-1, cols in 1..2^31-1"
+        _check_extents(rows, cols)
         q = MxFp4Tensor.__new__(MxFp4Tensor)
         q.storage = torch.empty(_units(rows, cols) * 2176, dtype=torch.uint8, device=device)
         q.rows, q.cols = rows, cols
@@ -124,7 +129,8 @@ class MxFp4Tensor:
         rows, blocks = scales.shape
         assert codes.shape[1] == blocks * (BLOCK // 2), "codes must have 16 bytes per block"
         cols = blocks * BLOCK if cols is None else int(cols)
-        assert blocks >= 1 and blocks == -(-cols // BLOCK), "cols must end in the last block"
+        assert blocks == -(-cols // BLOCK), "cols must end in the last block"
+        _check_extents(rows, cols)
         row_units, slabs = -(-rows // UNIT_ROWS), -(-cols // SLAB)
         padded = torch.zeros(row_units * UNIT_ROWS, slabs * SLAB // 2, dtype=torch.uint8, device=codes.device)
         used = -(-cols // 2)
@@ -208,7 +214,8 @@ def mxfp4_matmul(a: Union[MxFp4Tensor, torch.Tensor], b: MxFp4Tensor, *, out_dty
     """``a @ b.T`` for ``a`` [M, K] and ``b`` [N, K], accumulated in fp32 - in an order that depends
     on the sizes only - and rounded once to ``out_dtype`` (bf16 or fp32).  A bf16 or fp32 ``a`` is
     quantised on the way, as by :func:`mxfp4_quantize`; for up to 16 rows the order of the sum may
-    then be another.  ``out`` may not overlap an operand."""
+    then be another.  ``out`` may not overlap an operand.  K = 0 (a weight's gradient over no tokens)
+    gives zeros."""
     assert isinstance(b, MxFp4Tensor), "b must be an MxFp4Tensor"
     quantised = isinstance(a, MxFp4Tensor)
     shape = a.shape
@@ -226,6 +233,10 @@ def mxfp4_matmul(a: Union[MxFp4Tensor, torch.Tensor], b: MxFp4Tensor, *, out_dty
         assert out.device == device, "out must be on the operands' device"
         _check_apart(out, a.storage if quantised else a, b.storage)
         out_dtype = out.dtype
+    if b.cols == 0:
+        if not quantised:
+            _check_rows(a)
+        return out.zero_()
     lib = _lib.load()
     if not quantised:
         if M <= UNIT_ROWS and N <= _ROWS_MAX_N and M <= lib.smr_mxfp4_matmul_rows_limit(b.cols):

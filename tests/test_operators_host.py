@@ -191,3 +191,17 @@ def test_the_columns_of_the_few_rows_product_end_below_2_to_28(lib):
     assert f(p, 32, 0, p, p, p, 1, 2 ** 28 - 63, 32, 0, None) == -2
     assert b"columns" in lib.smr_last_error_string()
     assert f(p, 32, 0, p, p, p, 0, 2 ** 28 - 64, 32, 0, None) == 0               # no rows: no launch
+
+
+def test_operands_that_contract_over_nothing_on_the_host():
+    from symm_mem_recipes import MxFp4Tensor
+    none = torch.zeros(8, 0, dtype=torch.uint8)
+    q = MxFp4Tensor.from_blocks(none, none)
+    assert q.shape == (8, 0) and [t.shape for t in q.to_blocks()] == [(8, 0), (8, 0)]
+    assert MxFp4Tensor(torch.zeros(0, dtype=torch.uint8), 8, 0).shape == (8, 0)
+    assert MxFp4Tensor.empty(5, 0, "cpu").storage.numel() == 0
+    for rows, cols in ((0, 0), (-1, 4), (4, -1), (2 ** 31, 4), (4, 2 ** 31)):
+        with pytest.raises(AssertionError):
+            MxFp4Tensor.empty(rows, cols, "cpu")
+    with pytest.raises(AssertionError):
+        MxFp4Tensor.from_blocks(none[:0], none[:0])
