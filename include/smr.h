@@ -383,7 +383,8 @@ int smr_set_gemv_matrix_cores(int on);
  *   n = s * (mean(s^2) + eps)^-1/2 * post_weight              (post_weight NULL: n = s)
  *   h = residual_scale * residual + gate * n
  *   residual_out = h;  normed = h * (mean(h^2) + eps)^-1/2 * weight;  summed = s (NULL: not wanted)
- * Everything between the loads and the stores is fp32; each output is rounded once.
+ * Everything between the loads and the stores is fp32; each output is rounded once.  Rows whose squares leave fp32's
+ * range (magnitudes past 2^64, or below 2^-50 with an eps as small) are scaled by a power of two for their norms.
  *   buffer_ptrs_host, signal_pad_ptrs_host  HOST arrays, as in smr_one_shot_all_reduce_addrs
  *              (pads NULL allowed with SMR_BARRIER_NONE); every buffer holds rows * cols elements,
  *              each pad 4096 * world_size slots

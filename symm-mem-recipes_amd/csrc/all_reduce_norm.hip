@@ -49,13 +49,28 @@ __global__ __launch_bounds__(256) void all_reduce_norm_narrow_kernel(NormForward
       if (c < f.cols)
         for (int r = 0; r < f.world_size; ++r) v[c] += R::one((const void*)(uintptr_t)f.peers.p[r], at + c);
       sq += v[c] * v[c];
+      if (f.summed != nullptr && c < f.cols) R::put_one(f.summed, at + c, v[c]);
     }
-    const float r1 = f.post_weight != nullptr ? 1.0f / sqrtf(sq / (float)f.cols + f.eps) : 1.0f;
+    // (mean square + eps)^-1/2; v is scaled where its squares do not fit
+    auto reciprocal_root = [&]() {
+      float mean = sq / (float)f.cols + f.eps;
+      if (mean_out_of_range(mean)) {
+        const float by = mean_rescale(mean);
+        sq = 0.0f;
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          v[c] *= c < f.cols ? by : 0.0f;
+          sq += v[c] * v[c];
+        }
+        mean = sq / (float)f.cols + f.eps * by * by;
+      }
+      return 1.0f / sqrtf(mean);
+    };
+    const float r1 = f.post_weight != nullptr ? reciprocal_root() : 1.0f;
     sq = 0.0f;
 #pragma unroll
     for (int c = 0; c < N; ++c)
       if (c < f.cols) {
-        if (f.summed != nullptr) R::put_one(f.summed, at + c, v[c]);
         float n = v[c];
         if (f.post_weight != nullptr) n *= r1 * R::one(f.post_weight, c);
         if (f.gate_kind == kGateChannel) n *= R::one(f.gate, c);
@@ -65,7 +80,7 @@ __global__ __launch_bounds__(256) void all_reduce_norm_narrow_kernel(NormForward
         sq += v[c] * v[c];
         R::put_one(f.residual_out, at + c, v[c]);
       }
-    const float r2 = 1.0f / sqrtf(sq / (float)f.cols + f.eps);
+    const float r2 = reciprocal_root();
 #pragma unroll
     for (int c = 0; c < N; ++c)
       if (c < f.cols) R::put_one(f.normed, at + c, v[c] * r2 * R::one(f.weight, c));

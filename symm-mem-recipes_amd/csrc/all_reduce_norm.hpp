@@ -26,7 +26,7 @@ __global__ __launch_bounds__(THREADS) void all_reduce_norm_kernel(NormForward f,
   using R = Row<BF16>;
   constexpr int V = R::kVec;
   constexpr bool kKeepWeights = CHUNKS <= 2;
-  __shared__ float slots[2][THREADS / 64][1];
+  __shared__ float slots[3][THREADS / 64][1];
   const int waves = blockDim.x >> 6;
   const int cols = f.cols;
   const bool whole = WHOLE || cols == (int)blockDim.x * CHUNKS * V;
@@ -122,6 +122,24 @@ __global__ __launch_bounds__(THREADS) void all_reduce_norm_kernel(NormForward f,
       if constexpr (!AHEAD && CHUNKS > 1) __builtin_amdgcn_sched_barrier(0);
     }
   };
+  // (mean square + eps)^-1/2 of the row in s, whose sum of squares is sq; the row is scaled where its squares do not fit
+  auto reciprocal_root = [&]() __attribute__((always_inline)) {
+    float mean = sq[0] * inv_cols + f.eps;
+    // (the same bits in every thread: a scalar branch)
+    if (__builtin_expect(mean_out_of_range(__int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(mean)))), 0)) {
+      const float by = mean_rescale(mean);
+      sq[0] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[c][e] *= by;
+        count(c);
+      }
+      workgroup_sums<1>(sq, slots[2], waves);
+      mean = sq[0] * inv_cols + f.eps * by * by;
+    }
+    return 1.0f / sqrtf(mean);
+  };
   auto finish = [&](int64_t row) __attribute__((always_inline)) {
     const float token_gate = f.gate_kind == kGateToken ? own.token : 1.0f;
     if (f.summed != nullptr) {
@@ -131,7 +149,7 @@ __global__ __launch_bounds__(THREADS) void all_reduce_norm_kernel(NormForward f,
     float r1 = 1.0f;
     if (post) {
       workgroup_sums<1>(sq, slots[0], waves);
-      r1 = 1.0f / sqrtf(sq[0] * inv_cols + f.eps);
+      r1 = reciprocal_root();
     }
     sq[0] = 0.0f;
 #pragma unroll
@@ -146,7 +164,7 @@ __global__ __launch_bounds__(THREADS) void all_reduce_norm_kernel(NormForward f,
       put(f.residual_out, row, c);
     }
     workgroup_sums<1>(sq, slots[1], waves);
-    const float r2 = 1.0f / sqrtf(sq[0] * inv_cols + f.eps);
+    const float r2 = reciprocal_root();
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       if constexpr (!kKeepWeights) w[c] = R::load(f.weight, column(c), cols);

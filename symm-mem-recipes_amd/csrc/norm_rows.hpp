@@ -127,6 +127,14 @@ __device__ __forceinline__ void workgroup_sums(float (&v)[N], float (*slots)[N],
   for (int n = 0; n < N; ++n) v[n] = row16_sum(w < waves ? slots[w][n] : 0.0f);
 }
 
+// Squares leave fp32's range long before values do: past 2^64 they are infinite, below 2^-63 they lose bits.  A row
+// whose mean square (eps added) comes out outside [kLeastMean, infinity) is scaled by a power of two and its
+// squares are summed again; the factor drops out of v * (mean)^-1/2.  With up to 2^14 columns the scaled squares'
+// sum is in [2^-46, 2^110] one way and below 2^114 the other.
+constexpr float kLeastMean = 0x1p-100f;
+__device__ __forceinline__ bool mean_out_of_range(float mean) { return !(mean >= kLeastMean && mean < __builtin_inff()); }
+__device__ __forceinline__ float mean_rescale(float mean) { return mean < kLeastMean ? 0x1p100f : 0x1p-80f; }
+
 // Threads and 128-bit chunks per thread for a row; the smallest number of chunks that fits.
 inline bool norm_shape(int cols, int vec, int max_threads, int& threads, int& chunks) {
   for (chunks = 1; chunks <= 8; chunks *= 2) {
