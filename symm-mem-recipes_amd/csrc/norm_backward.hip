@@ -37,7 +37,7 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward f) 
   constexpr bool kKeep = USE != kReread;
   constexpr int kHeld = kKeep ? CHUNKS : 1;
   __shared__ u32x4 weights[2][kKeep ? CHUNKS * THREADS : 1];      // a thread's own vectors of weight and post_weight
-  __shared__ float slots3[THREADS / 64][3], slots2[THREADS / 64][2];
+  __shared__ float slots3[2][THREADS / 64][3], slots2[THREADS / 64][2];
   const int waves = blockDim.x >> 6;
   const int cols = f.cols;
   const bool whole = WHOLE || cols == (int)blockDim.x * CHUNKS * V;
@@ -94,16 +94,20 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward f) 
     if constexpr (kKeep) return weights[which][c * THREADS + threadIdx.x];
     else return R::load(which == 0 ? f.weight : post_weight, column(c), cols);
   };
-  // Column sums of the workgroup's rows.
-  float sum_w[kHeld][V], sum_p[kHeld][V], sum_g[kHeld][V];
+  // Column sums of the workgroup's rows: the weight's, and D * s * r1 times the gate.  With a gate per channel the gate
+  // stays out: the sum is the post weight's but for the gate and the gate's but for the post weight.
+  const bool channel = f.gate_kind == kGateChannel;
+  float sum_w[kHeld][V], sum_n[kHeld][V];
 #pragma unroll
   for (int c = 0; c < kHeld; ++c)
 #pragma unroll
-    for (int e = 0; e < V; ++e) sum_w[c][e] = sum_p[c][e] = sum_g[c][e] = 0.0f;
+    for (int e = 0; e < V; ++e) sum_w[c][e] = sum_n[c][e] = 0.0f;
 
   In in;
   float t[3];                                 // sums of h^2, dy*weight*h, s^2
-  auto begin = [&](int64_t row) __attribute__((always_inline)) {
+  // (SCALED: of h and s times a factor each, for rows whose squares do not fit fp32)
+  auto row_sums = [&](auto scaled, int64_t row, float by_h, float by_s) __attribute__((always_inline)) {
+    constexpr bool SCALED = decltype(scaled)::value;
     // (recomputed for every row: kept, the addresses of all chunks would take the sums' registers)
     if constexpr (USE != kAhead) asm volatile("" : "+v"(tid));
     t[0] = t[1] = t[2] = 0.0f;
@@ -116,7 +120,7 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward f) 
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         // (the products are masked, not their factors: another vector's infinity must not become a NaN here)
-        const float he = R::get(in.h[k], e), se = R::get(in.s[k], e);
+        const float he = R::get(in.h[k], e) * (SCALED ? by_h : 1.0f), se = R::get(in.s[k], e) * (SCALED ? by_s : 1.0f);
         const bool own = e >= first;
         t[0] += own ? he * he : 0.0f;
         t[1] += own ? R::get(in.dy[k], e) * R::get(w, e) * he : 0.0f;
@@ -127,15 +131,28 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward f) 
       if constexpr (!kKeep) __builtin_amdgcn_sched_barrier(0);
     }
   };
+  auto begin = [&](int64_t row) __attribute__((always_inline)) { row_sums(std::false_type{}, row, 1.0f, 1.0f); };
   auto finish = [&](int64_t row) __attribute__((always_inline)) {
     if constexpr (USE != kAhead) asm volatile("" : "+v"(tid));
     const float token_gate = f.gate_kind == kGateToken ? in.token : 1.0f;
-    workgroup_sums<3>(t, slots3, waves);
-    const float r2 = 1.0f / sqrtf(t[0] * inv_cols + f.eps);
-    const float along = t[1] * inv_cols * r2 * r2;
-    const float r1 = post ? 1.0f / sqrtf(t[2] * inv_cols + f.eps) : 1.0f;
+    workgroup_sums<3>(t, slots3[0], waves);
+    float mean_h = t[0] * inv_cols + f.eps, mean_s = t[2] * inv_cols + f.eps, by_h = 1.0f, by_s = 1.0f;
+    const bool odd_h = mean_out_of_range(mean_h), odd_s = post && mean_out_of_range(mean_s);
+    // (the same in every thread: a scalar branch)
+    if (__builtin_expect(__any(odd_h || odd_s), 0)) {
+      by_h = odd_h ? mean_rescale(mean_h) : 1.0f;
+      by_s = odd_s ? mean_rescale(mean_s) : 1.0f;
+      row_sums(std::true_type{}, row, by_h, by_s);
+      workgroup_sums<3>(t, slots3[1], waves);
+      mean_h = t[0] * inv_cols + f.eps * by_h * by_h;
+      mean_s = t[2] * inv_cols + f.eps * by_s * by_s;
+    }
+    const float root_h = 1.0f / sqrtf(mean_h);
+    const float r2 = root_h * by_h;
+    const float along = t[1] * inv_cols * root_h * r2;
+    const float r1 = post ? 1.0f / sqrtf(mean_s) * by_s : 1.0f;
     float d[kKeep ? CHUNKS : 1][V];           // dn*post_weight
-    float u[2] = {0.0f, 0.0f};                // sums of dn*post_weight*s and D*n
+    float u[2] = {0.0f, 0.0f};                // sums of dn*post_weight*s*r1 and D*n
     // D of an element
     auto whole_gradient = [&](int k, int e, const u32x4& w) __attribute__((always_inline)) {
       const float he = R::get(in.h[k], e), dye = R::get(in.dy[k], e);
@@ -150,14 +167,14 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward f) 
       float out[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float D = whole_gradient(k, e, w), se = R::get(in.s[k], e);
+        // (h and s meet their reciprocal root first: a product of theirs with a gradient may be out of range)
+        const float D = whole_gradient(k, e, w), se = R::get(in.s[k], e) * r1;
         out[e] = f.residual_scale * D;
-        const float pe = post ? R::get(p, e) : 1.0f, dg = D * (se * r1 * pe);
+        const float pe = post ? R::get(p, e) : 1.0f, dg = D * (se * pe);
         const float dn = D * (gated ? R::get(in.g[k], e) : token_gate);
         if constexpr (kKeep) {
-          sum_w[c][e] += R::get(in.dy[k], e) * R::get(in.h[k], e) * r2;
-          sum_g[c][e] += dg;
-          sum_p[c][e] += dn * se * r1;
+          sum_w[c][e] += R::get(in.dy[k], e) * (R::get(in.h[k], e) * r2);
+          sum_n[c][e] += (channel ? D : dn) * se;
         }
         const float dnp = dn * pe;
         if constexpr (kKeep) d[c][e] = dnp;
@@ -181,7 +198,7 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward f) 
     }
     workgroup_sums<2>(u, slots2, waves);
     if (f.gate_kind == kGateToken && threadIdx.x == 0) R::put_one(f.grad_gate, row, u[1]);
-    const float back = u[0] * inv_cols * r1 * r1;
+    const float back = u[0] * inv_cols * r1;
     if constexpr (!kKeep)
       if (threadIdx.x == 0) {
         f.row_values[row * 3] = r2;
@@ -239,13 +256,21 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward f) 
       }
     };
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
+    for (int c = 0; c < CHUNKS; ++c) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        put_sum(sum_w[c][e], c, e, 0);
-        if (post) put_sum(sum_p[c][e], c, e, 1);
-        if (f.gate_kind == kGateChannel) put_sum(sum_g[c][e], c, e, post ? 2 : 1);
+      for (int e = 0; e < V; ++e) put_sum(sum_w[c][e], c, e, 0);
+      if (channel) {
+        const u32x4 p = weight_of(1, c), g = R::load(gate, column(c), cols);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          put_sum(post ? sum_n[c][e] * R::get(p, e) : sum_n[c][e], c, e, post ? 2 : 1);
+          if (post) put_sum(sum_n[c][e] * R::get(g, e), c, e, 1);
+        }
+      } else if (post) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) put_sum(sum_n[c][e], c, e, 1);
       }
+    }
   }
 }
 
@@ -284,8 +309,8 @@ __global__ __launch_bounds__(64) void norm_columns_kernel(NormBackward f) {
     for (int e = 0; e < V; ++e) {
       const float he = R::get(h, e), dye = R::get(dy, e), se = R::get(s, e);
       const float D = (has_dh ? R::get(dh, e) : 0.0f) + r2 * (dye * R::get(w, e) - he * along);
-      sums[0][e] += dye * he * r2;
-      sums[1][e] += D * (gated ? R::get(g, e) : token_gate) * se * r1;
+      sums[0][e] += dye * (he * r2);
+      sums[1][e] += D * (gated ? R::get(g, e) : token_gate) * (se * r1);
       sums[2][e] += D * (se * r1 * (post ? R::get(p, e) : 1.0f));
     }
   }
@@ -324,31 +349,45 @@ __global__ __launch_bounds__(256) void norm_backward_narrow_kernel(NormBackward 
       dyh += R::one(f.grad_normed, at + c) * R::one(f.weight, c) * h;
       s2 += s * s;
     }
-    const float r2 = 1.0f / sqrtf(h2 * inv_cols + f.eps), along = dyh * inv_cols * r2 * r2;
-    const float r1 = post ? 1.0f / sqrtf(s2 * inv_cols + f.eps) : 1.0f;
+    float mean_h = h2 * inv_cols + f.eps, mean_s = s2 * inv_cols + f.eps, by_h = 1.0f, by_s = 1.0f;
+    if (mean_out_of_range(mean_h) || (post && mean_out_of_range(mean_s))) {
+      by_h = mean_out_of_range(mean_h) ? mean_rescale(mean_h) : 1.0f;
+      by_s = mean_out_of_range(mean_s) ? mean_rescale(mean_s) : 1.0f;
+      h2 = dyh = s2 = 0.0f;
+      for (int c = 0; c < f.cols; ++c) {
+        const float h = R::one(f.residual_out, at + c) * by_h, s = R::one(f.summed, at + c) * by_s;
+        h2 += h * h;
+        dyh += R::one(f.grad_normed, at + c) * R::one(f.weight, c) * h;
+        s2 += s * s;
+      }
+      mean_h = h2 * inv_cols + f.eps * by_h * by_h;
+      mean_s = s2 * inv_cols + f.eps * by_s * by_s;
+    }
+    const float root_h = 1.0f / sqrtf(mean_h), r2 = root_h * by_h, along = dyh * inv_cols * root_h * r2;
+    const float r1 = post ? 1.0f / sqrtf(mean_s) * by_s : 1.0f;
     float d[N], dns = 0.0f, token = 0.0f;
 #pragma unroll
     for (int c = 0; c < N; ++c)
       if (c < f.cols) {
-        const float h = R::one(f.residual_out, at + c), s = R::one(f.summed, at + c), dy = R::one(f.grad_normed, at + c);
+        const float h = R::one(f.residual_out, at + c), s = R::one(f.summed, at + c) * r1, dy = R::one(f.grad_normed, at + c);
         const float D = (f.grad_residual_out != nullptr ? R::one(f.grad_residual_out, at + c) : 0.0f) +
                         r2 * (dy * R::one(f.weight, c) - h * along);
-        const float p = post ? R::one(f.post_weight, c) : 1.0f, dg = D * s * r1 * p;
+        const float p = post ? R::one(f.post_weight, c) : 1.0f, dg = D * (s * p);
         float g = 1.0f;
         if (f.gate_kind == kGateChannel) g = R::one(f.gate, c);
         if (f.gate_kind == kGateToken) g = R::one(f.gate, row);
         if (f.gate_kind == kGateElement) g = R::one(f.gate, at + c);
         if (f.gate_kind == kGateElement) R::put_one(f.grad_gate, at + c, dg);
         R::put_one(f.grad_residual, at + c, f.residual_scale * D);
-        sums[0][c] += dy * h * r2;
-        sums[1][c] += D * g * s * r1;
+        sums[0][c] += dy * (h * r2);
+        sums[1][c] += D * g * s;
         sums[2][c] += dg;
         token += dg;
         d[c] = D * g * p;
         dns += d[c] * s;
       }
     if (f.gate_kind == kGateToken) R::put_one(f.grad_gate, row, token);
-    const float back = dns * inv_cols * r1 * r1;
+    const float back = dns * inv_cols * r1;
 #pragma unroll
     for (int c = 0; c < N; ++c)
       if (c < f.cols) R::put_one(f.grad_partial, at + c, post ? r1 * (d[c] - R::one(f.summed, at + c) * back) : d[c]);

@@ -67,3 +67,47 @@ def test_ordinary_rows_beside_large_ones_keep_their_bits(cuda):
         for got, want in zip(one_shot_all_reduce_norm(t, x, w, post_weight=p, gate=gc, return_sum=True), plain):
             assert torch.equal(got[keep], want[keep])
         SM.release()
+
+
+BACKWARD_SHAPES = [((7, 5), "bf16"), ((7, 3), "fp32"), ((9, 200), "bf16"), ((4, 1001), "fp32"), ((530, 8192), "bf16"),
+                   ((261, 8001), "bf16"), ((270, 4096), "fp32"), ((265, 8191), "fp32"), ((5, 16384), "bf16"), ((4, 9001), "fp32"),
+                   ((600, 512), "bf16")]
+
+
+@pytest.mark.parametrize("post", [True, False])
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "element"])
+@pytest.mark.parametrize("shape,dtype", BACKWARD_SHAPES)
+def test_backward_over_the_range_of_the_type(cuda, shape, dtype, gate, post):
+    """The forward pass's sums and outputs are large or small in every third row.  The bound on the terms of a
+    gradient is that of ordinary rows (at most 128 roundings, and the terms of a column sum): scaling by a power of two
+    rounds nothing, a subnormal reciprocal root (rows past 2^126) does not occur."""
+    from symm_mem_recipes import one_shot_all_reduce_norm_backward
+    from tests.test_gpu_all_reduce_norm import _backward_inputs
+    dtype = DTYPES[dtype]
+    dy, dh, s, h, w, p, g = _backward_inputs(shape, dtype, post, gate, True, sum(shape) + 5)
+    rows = shape[0]
+    for sizes, eps in (((LARGE, 2.0 ** 115), 1e-6), ((1e-16, LARGE), 0.0)):
+        factors = _factors(rows, sizes)
+        # (without the norm behind the block the gate's gradient has the sums as a factor: D times them may pass the type)
+        hs, ss = _scaled(h, factors, 0), _scaled(s, factors.flip(0) if post else torch.ones_like(factors), 0)
+        args = (dy, dh, ss, hs, w, p, g, 1.0, eps)
+        a = _cuda(*args[:7])
+        got = one_shot_all_reduce_norm_backward(a[0], a[1], a[2], a[3], a[4], post_weight=a[5], gate=a[6], eps=eps)
+        want, size = oracle.backward(*args), oracle.backward(*args, magnitudes=True)
+        for name, b in want.items():
+            off = size[name] * (128 + rows / 128 + 64) * oracle.U
+            _within(getattr(got, name).reshape(b.shape), b, off, dtype)
+
+
+def test_gradients_of_ordinary_rows_beside_large_ones_keep_their_bits(cuda):
+    from symm_mem_recipes import one_shot_all_reduce_norm_backward
+    from tests.test_gpu_all_reduce_norm import _backward_inputs
+    for shape in ((301, 8192), (9, 1000), (8, 6), (6, 12000)):
+        dy, dh, s, h, w, p, g = _cuda(*_backward_inputs(shape, torch.bfloat16, True, "element", True, 9))
+        plain = one_shot_all_reduce_norm_backward(dy, dh, s, h, w, post_weight=p, gate=g)
+        factors = _factors(shape[0], (LARGE,)).cuda()
+        keep = factors == 1
+        large = [torch.where(keep[:, None], t, (t.double() * factors[:, None]).bfloat16()) for t in (s, h)]
+        got = one_shot_all_reduce_norm_backward(dy, dh, *large, w, post_weight=p, gate=g)
+        for name in ("partial", "residual", "gate"):
+            assert torch.equal(getattr(got, name)[keep], getattr(plain, name)[keep]), name
