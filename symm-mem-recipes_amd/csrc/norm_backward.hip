@@ -437,11 +437,21 @@ __global__ __launch_bounds__(kSumThreads) void norm_sums_kernel(const float* __r
   }
 }
 
-// Rows that one workgroup takes, one after the other, instead of one workgroup each and a second launch for
-// their sums: 3 x 4096 8.0 us and 7.8, 5 x 4096 11.0 and 7.7 - but the second launch and its scratch array
-// cost a caller on the host another 4.4 us.  (As many rows at a time as 1024 threads have room for, their sums
-// joined in LDS: 16 x 512 10.4 us against 6.4 in two launches, 40 x 1000 30 against 8.2.)
-constexpr int kOneWorkgroupRows = 5;
+// Rows that one workgroup takes, one after the other, instead of one workgroup each and a second launch for their sums.
+// The second launch and its scratch array cost the host 4 us (12.4 us a call, 16.4 with them), so one workgroup is
+// taken while it is slower on the GPU by no more than that.  A row's time grows with its width: times on the GPU, one
+// workgroup / two launches, in us:
+//     rows          2            3            4            5            8
+//    512 bf16    5.3 /  6.1   6.4 /  6.0   7.5 /  6.1   8.7 /  6.1  12.0 /  6.1    one vector a thread
+//   2048 fp32    5.9 /  6.7   7.3 /  6.7   8.7 /  6.8  10.2 /  6.8                 one
+//   4096 bf16    7.7 /  9.8   9.5 /  9.9  11.3 /  9.8  13.2 /  9.9  18.7 /  9.9    one
+//   8192 bf16   11.2 / 14.6  13.9 / 14.7  16.6 / 14.7  19.3 / 14.7                 two
+//   8192 fp32   12.9 / 11.8  16.6 / 11.9               23.9 / 11.9                 two, 1024 threads
+// Where the host has no part in it, in a replayed graph, two launches would do better from three or four rows on; a
+// single call that is waited for breaks even at four (4 x 4096 29.5 us and 29.7, 5 x 4096 31.7 and 30.1).
+// (As many rows at a time as 1024 threads have room for, their sums joined in LDS: 16 x 512 10.4 us against 6.4 in two
+// launches, 40 x 1000 30 against 8.2.)
+static int one_workgroup_rows(int threads, int chunks) { return threads > 512 ? 2 : (chunks == 1 ? 5 : 4); }
 
 // How a backward pass is launched; `parts` > 1 leave cols fp32 sums per kind each.
 struct BackwardShape {
@@ -459,7 +469,7 @@ static BackwardShape backward_shape(int64_t rows, int cols, bool bf16) {
   }
   if (s.wide) {
     s.parts = (int)(rows < 128 ? rows : 128);
-  } else if (rows > kOneWorkgroupRows) {
+  } else if (rows > one_workgroup_rows(s.threads, s.chunks)) {
     const int64_t most = 256 * (int64_t)(s.threads <= 256 ? 512 / s.threads : 1);
     s.parts = (int)(rows < most ? rows : most);
   }

@@ -205,3 +205,12 @@ def test_operands_that_contract_over_nothing_on_the_host():
             MxFp4Tensor.empty(rows, cols, "cpu")
     with pytest.raises(AssertionError):
         MxFp4Tensor.from_blocks(none[:0], none[:0])
+
+
+def test_rows_that_one_workgroup_takes_depend_on_their_width(lib):
+    """Up to how many rows the norms' backward pass needs no scratch array: fewer the more vectors a thread has."""
+    def single(cols, dtype):
+        return max(r for r in range(1, 65) if lib.smr_norm_backward_scratch_bytes(r, cols, dtype, 1, 1) == 0)
+
+    assert [single(c, 0) for c in (64, 4096, 4097, 8192)] == [5, 5, 4, 4]
+    assert [single(c, 1) for c in (64, 2048, 2049, 4096, 4097, 8192)] == [5, 5, 4, 4, 2, 2]
