@@ -804,7 +804,14 @@ struct MxRows {
   uint8_t* c;
   int64_t M, N, K;
 };
-// Rows times slabs whose codes and scales (136 B each) fit a workgroup's LDS beside the partial sums.
+// Rows times slabs of one launch: their codes and scales (136 B each) and 32 KiB of partial sums are half of a compute
+// unit's LDS, so that two workgroups fit.  Quantising takes a workgroup longer the more there are, and with one
+// workgroup per compute unit wide results wait for it; K = 8192, us of one launch / quantiser and product:
+//   rows (units)   8 (256)        11 (352)       12 (384)       16 (512)
+//   N =  3584     8.3 /  8.0     9.3 /  8.1     9.7 /  8.2    11.1 /  8.1
+//   N =  8192    10.4 / 10.8    11.1 / 10.8    11.5 / 10.8    12.6 / 10.9
+//   N = 28672    28.4 / 26.3    29.1 / 26.1    33.0 / 24.9    35.8 / 25.3
+// Up to there the second launch would cost a caller on the host (4 us) more than one launch costs the GPU.
 constexpr int kRowsLdsUnits = 352;
 // Columns that one launch of four units of columns per workgroup takes.
 constexpr int64_t kRowsMaxN = kMxMaxGrid / 4 * 4 * kMxRows;

@@ -168,7 +168,8 @@ def test_product(cuda, M, N, K, out_dtype):
     assert torch.equal(mxfp4_matmul(a, qb, out_dtype=out_dtype), direct)
 
 
-# (each of the matrix-tile kernels, one pass over the chip and several; odd widths, units and tiles that end early)
+# (each of the matrix-tile kernels, one pass over the chip and several - the 256 x 128 tile one pass, several are in
+# test_gpu_mxfp4_launches.py; odd widths, units and tiles that end early)
 LARGE = [(300, 3000, 900), (1500, 3500, 1100), (1100, 3001, 700), (2049, 3585, 900), (2000, 3300, 1000), (4097, 3585, 700),
          (4000, 3584, 1100), (4200, 7201, 1000), (4090, 7161, 1300), (5003, 7392, 257),
          (512, 3583, 1500), (700, 2001, 700), (4001, 4090, 1111), (8003, 4081, 700), (8200, 2050, 1300)]
