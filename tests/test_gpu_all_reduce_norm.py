@@ -186,7 +186,7 @@ BACKWARD = [
     ((2, 8200), "bf16", True, "element", 1.0, True), ((2, 16384), "bf16", True, "channel", 1.0, True),
     ((2, 16383), "bf16", True, "token", 1.0, True), ((2, 16381), "fp32", True, "channel", 1.0, True),
     ((1030, 2048), "bf16", True, "token", 1.0, True), ((5000, 40), "fp32", True, "element", 1.0, True),
-    # one workgroup, several rows at a time, the last turn full and not
+    # a few rows more than one workgroup takes: a workgroup each and a second launch for their sums (5 x 1536: one workgroup)
     ((80, 512), "bf16", True, "channel", 1.0, True), ((79, 499), "bf16", True, "token", 1.0, False), ((40, 1000), "bf16", False, "channel", 1.0, True),
     ((33, 777), "bf16", True, "element", 2.0, True), ((20, 2048), "bf16", True, "none", 1.0, True), ((10, 4001), "bf16", True, "channel", 1.0, True),
     ((65, 250), "fp32", True, "channel", 1.0, True), ((17, 300), "fp32", False, "token", 1.0, True), ((9, 2048), "fp32", True, "element", 1.0, False),
@@ -208,6 +208,8 @@ def _backward_inputs(shape, dtype, post, gate, with_dh, seed):
     return dy, dh if with_dh else None, s * 2, h, weight, post_weight, g
 
 
+# (With up to 2048 workgroups, 5000 x 40, a thread of the summing kernel adds 64 of their sums, not 32: 3 terms in a
+# workgroup, 64 and 32 are 99, and the bound has 5000 / 128 + 64 = 103.)
 @pytest.mark.parametrize("shape,dtype,post,gate,scale,with_dh", BACKWARD)
 def test_backward(cuda, shape, dtype, post, gate, scale, with_dh):
     """Every term of a gradient passes through at most 128 roundings on its way (32 values and 22
