@@ -8,6 +8,7 @@ package's entry points (``own`` true) from the same inputs, which ``prepare`` ma
 """
 import math
 import sys
+import weakref
 
 import torch
 
@@ -137,7 +138,10 @@ def prepare(case, seed):
         if own:
             symm = package().EmulatedSymmetricMemory
             tensor = symm.empty_strided_p2p((T, H), (H, 1), dtype, "cuda", world_size=case["ranks"], rank=0)
-            symm.rendezvous(tensor).all_buffers((T, H), dtype).copy_(partials)
+            handle = symm.rendezvous(tensor)
+            handle.all_buffers((T, H), dtype).copy_(partials)
+            # the registry of symmetric allocations would keep this one beyond its state
+            weakref.finalize(tensor, symm.release, handle.get_buffer(0, (T, H), dtype)).atexit = False
             state["tensor"] = tensor
         else:
             state["partials"] = partials
