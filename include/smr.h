@@ -390,7 +390,9 @@ int smr_set_gemv_matrix_cores(int on);
  *              each pad 4096 * world_size slots
  *   dtype      SMR_DTYPE_BF16 or _FP32, of all tensors; rows are contiguous, cols in 1..16384
  *   gate_kind  0 none (gate NULL), 1 one per column [cols], 2 one per row [rows], 3 [rows, cols]
- *   barrier_mode  SMR_BARRIER_NONE or _PROXY.  residual_out may be residual. */
+ *   barrier_mode  SMR_BARRIER_NONE or _PROXY: the handshake in front of the reads; none follows them, so a buffer is
+ *              overwritten only behind its peers' calls.
+ * residual_out may be residual; all else that is written lies apart from what is read. */
 int smr_all_reduce_norm(const uint64_t* buffer_ptrs_host, const uint64_t* signal_pad_ptrs_host, const void* residual,
                         const void* weight, const void* post_weight, const void* gate, int gate_kind, void* normed,
                         void* residual_out, void* summed, int64_t rows, int64_t cols, int dtype, double residual_scale,
@@ -400,7 +402,9 @@ int smr_all_reduce_norm(const uint64_t* buffer_ptrs_host, const uint64_t* signal
  * two outputs (grad_residual_out NULL: zero).  grad_partial is the gradient of every rank's
  * partial sums.  Gradients of the weights and of a broadcast gate are summed over what they were
  * broadcast over, in fp32 and in an order that depends on the sizes only.
- *   scratch    smr_norm_backward_scratch_bytes(...) bytes (NULL where that is 0); needs no initialisation */
+ *   scratch    smr_norm_backward_scratch_bytes(...) bytes (NULL where that is 0); needs no initialisation
+ * What is written lies apart from what is read: rows are read more than once.  Rows narrower than 16 bytes go through
+ * one workgroup, 22 us per 1000 of them. */
 int smr_norm_backward(const void* grad_normed, const void* grad_residual_out, const void* summed,
                       const void* residual_out, const void* weight, const void* post_weight, const void* gate,
                       int gate_kind, void* grad_partial, void* grad_residual, void* grad_weight,
@@ -428,7 +432,8 @@ int64_t smr_mxfp4_scale_bytes(int64_t rows, int64_t cols);
  *   saturate at 6 scales.  A block that holds an infinity or a NaN becomes NaN (scale code 255). */
 int smr_mxfp4_quantize(const void* x_dev, int64_t row_stride, void* codes_dev, void* scales_dev, int64_t rows,
                        int64_t cols, int dtype, int transpose, void* stream);
-/* The values an operand stands for, [rows, cols] contiguous bf16 or fp32 (exact in both). */
+/* The values an operand stands for, [rows, cols] contiguous bf16 or fp32: exact in both, but for values past both types
+ * (scale codes 253 and 254, which the quantiser does not write), which become infinite. */
 int smr_mxfp4_dequantize(const void* codes_dev, const void* scales_dev, void* out_dev, int64_t rows, int64_t cols,
                          int dtype, void* stream);
 

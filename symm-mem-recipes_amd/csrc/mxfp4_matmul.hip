@@ -252,7 +252,7 @@ __global__ __launch_bounds__(WAVES * 64) void mxfp4_matmul_rows_kernel(
 //   barrier       pair kt is read by everyone, pair kt+1 has landed
 //   second step   MFMAs of step 1; fragments of step 0 and the scales of pair kt+1 are read;
 //                 B slab and scales of pair kt+2 (and its A slab where LDS holds two) are requested
-// 16384 x 3584 x 8192: 201 us, 4.8 PFLOP/s.  Nothing but its MFMAs on such data takes 149 us (6.5 PFLOP/s: the
+// 16384 x 3584 x 8192: 201-205 us, 4.7-4.8 PFLOP/s.  Nothing but its MFMAs on such data takes 149 us (6.5 PFLOP/s: the
 // clock is power-limited; zeros reach 8.9).  With 32 bytes a row per store it took 224: 187 without the stores, 190
 // without the loads from memory, 178 without those and the fragment reads.  Stores that stay in flight under the next
 // tile's first slabs, and 128 bytes a row per store, were no faster than 64.
@@ -652,8 +652,9 @@ __global__ __launch_bounds__(kTileThreads, 1) void mxfp4_matmul_tile_kernel(MxTi
 // ---------------------------------------------------------------------------
 // The same product in smaller tiles, for results that have too few of the large ones to fill the
 // chip.  What bounds those is the arrival of the slabs - first the latency, then the 62 bytes/ns that a compute
-// unit receives (64 x 128: 26 KB per slab pair in 0.42 us) - so LDS holds BUFFERS whole slab pairs and all but the
-// two being multiplied and read are on their way; the order inside a pair is the compiler's.  Three: two workgroups
+// unit takes in, four fifths of them L2 hits (64 x 128: 26 KB per slab pair in 0.42 us) - so LDS holds BUFFERS whole
+// slab pairs and all but the two being multiplied and read are on their way; the order inside a pair is the compiler's.
+// Three: two workgroups
 // fit a compute unit (1500 x 3500 x 1100: 11.9 us, with four 14.6), and alone four to six are no faster (1001 x
 // 1777 x 4000: 11.8, 12.0, 12.3, 12.4), nor is a second group of waves that takes every other slab (12.2).
 // One tile per workgroup.

@@ -82,7 +82,7 @@ def one_shot_all_reduce_norm(tensor: torch.Tensor, residual: torch.Tensor, weigh
         normed       = residual_out * rsqrt(mean(residual_out ** 2) + eps) * weight
 
     with means over the last dimension, everything in fp32 and each output rounded once (the
-    norms are of the unrounded values).
+    norms are of the unrounded values; rows whose squares do not fit fp32 are scaled for them).
 
     ``tensor``    partial sums [..., cols], allocated via SymmetricMemory, bf16 or fp32, cols <= 16384
     ``residual``  of the same shape and dtype
@@ -90,7 +90,8 @@ def one_shot_all_reduce_norm(tensor: torch.Tensor, residual: torch.Tensor, weigh
     ``gate``      [cols] (one per channel), [..., 1] (one per token) or of ``tensor``'s shape; a
                   one-dimensional gate of a one-dimensional tensor is per channel
     ``barrier``   the blockwise handshake before the peers are read, as one_shot_all_reduce, and on the
-                  same signal pads: calls on one allocation belong on one stream at a time
+                  same signal pads: calls on one allocation belong on one stream at a time.  None follows
+                  the reads: a rank overwrites its buffer only behind its peers' calls
     ``return_sum`` keep the sum too: the backward pass needs it
     """
     rows, cols, kind = _check(tensor, weight, post_weight, gate, residual)
@@ -119,7 +120,7 @@ def one_shot_all_reduce_norm_backward(grad_normed: torch.Tensor, grad_residual_o
     gradients of ``normed`` and ``residual_out`` (None: zero) and from the forward pass's
     ``summed`` and ``residual_out``; the other arguments as given there.  The gradients of the
     weights and of a broadcast gate are summed in fp32, in an order that depends on the sizes
-    only, and rounded once."""
+    only, and rounded once.  Rows narrower than 16 bytes go through one workgroup (22 us per 1000)."""
     same = (summed, residual_out) if grad_residual_out is None else (grad_residual_out, summed, residual_out)
     rows, cols, kind = _check(grad_normed, weight, post_weight, gate, *same)
     grads = NormGradients(torch.empty_like(grad_normed), torch.empty_like(grad_normed), torch.empty_like(weight),

@@ -1,7 +1,8 @@
 """4-bit microscaled operands (OCP MXFP4: e2m1 elements, one power-of-two scale per 32 of
 them along the contracted axis): quantisation, the values back, and the product of two
-operands.  The next narrower form of the e4m3fn switch of the all-gather matmul
-(symm_mem_recipes/triton_all_gather_matmul.py:115,123,188), which has no 4-bit form.
+operands.  The next narrower type after the e4m3fn switch of the all-gather matmul
+(symm_mem_recipes/triton_all_gather_matmul.py:115,123,188); that product takes no 4-bit operands, this one multiplies
+what one GPU holds.
 
 For training, the two products of a linear layer's backward pass contract over the layer's
 outputs and over the tokens; ``mxfp4_quantize(..., transpose=True)`` gives their operands::
@@ -154,7 +155,8 @@ class MxFp4Tensor:
                 scales.reshape(row_units * UNIT_ROWS, slabs * 8)[:self.rows, :blocks].contiguous())
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """The values, ``[rows, cols]`` bf16 or fp32 (exact in both)."""
+        """The values, ``[rows, cols]`` bf16 or fp32: exact in both, but for those of a checkpoint's scale codes 253 and
+        254 that are past both types and become infinite."""
         storage = self.storage
         if out is None:
             assert dtype in _DTYPE_CODE, "Only bfloat16 and float32 are supported for now."
