@@ -108,3 +108,31 @@ def test_no_base_of_an_assembly_load_is_written_by_a_vector_instruction_right_be
                     bad.append((name, writer, ins.text))
     assert seen > 20
     assert not bad, (len(bad), bad[:3])
+
+
+def test_no_result_of_an_assembly_mfma_is_touched_right_behind_it(compiled):
+    """A vector instruction that reads or writes an MFMA's result has to be up to 19 wait states behind it (16
+    passes); the kernels leave 32 in front of their epilogue, and nothing of the compiler's may come sooner."""
+    seen, bad = 0, []
+    for name, (code, labels) in compiled.items():
+        for i, ins in enumerate(code):
+            if not (ins.in_assembly and ins.op.startswith("v_mfma")):
+                continue
+            seen += 1
+            result, todo, visited = ins.registers[0], [(i + 1, 0)], set()
+            while todo:
+                j, passed = todo.pop()
+                if j >= len(code) or passed >= 19 or (j, passed) in visited:
+                    continue
+                visited.add((j, passed))
+                if code[j].vector and set().union(*code[j].registers) & result:
+                    bad.append((name, ins.text, code[j].text))
+                    break
+                if code[j].op == "s_endpgm":
+                    continue
+                if code[j].target in labels:
+                    todo.append((labels[code[j].target], passed + code[j].states))
+                if code[j].op != "s_branch":
+                    todo.append((j + 1, passed + code[j].states))
+    assert seen > 100
+    assert not bad, (len(bad), bad[:3])
